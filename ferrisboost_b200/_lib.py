@@ -68,6 +68,13 @@ class FbgpuSplit(C.Structure):
     ]
 
 
+class FbgpuSampleParams(C.Structure):
+    _fields_ = [
+        ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+        ("temperatures", P), ("top_ks", P), ("top_ps", P), ("min_ps", P),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     # include/fbgpu.h
@@ -112,6 +119,15 @@ SIGNATURES = {
     "fbgpu_shap_device": (C.c_int, [P, P, C.c_uint64, P, P]),
     "fbgpu_explain": (C.c_int, [P, C.c_int32, f32p, C.c_uint64, f32p]),
     "fbgpu_explain_device": (C.c_int, [P, C.c_int32, P, C.c_uint64, P, P]),
+    "fbgpu_embed": (C.c_int, [P, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, P, C.c_int32, C.c_uint64, C.c_uint32,
+                              C.c_uint64, C.c_uint64, C.c_float, P, C.c_uint64, P]),
+    "fbgpu_embed_grad_workspace": (C.c_uint64, [C.c_uint64, C.c_uint32, C.c_uint64, C.c_uint32]),
+    "fbgpu_embed_grad": (C.c_int, [P, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint64, P, C.c_int32,
+                                   C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, P, C.c_uint64, P, C.c_uint64, P]),
+    "fbgpu_dropout": (C.c_int, [P, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint64, C.c_double, C.c_uint64,
+                                C.c_uint64, P, C.c_uint64, P]),
+    "fbgpu_sample": (C.c_int, [P, C.c_int32, C.c_uint64, C.c_uint32, C.c_uint64, P, C.POINTER(FbgpuSampleParams), P,
+                               P, P]),
     # include/fb_engine.h
     "fb_default_params": (None, [C.POINTER(FbParams)]),
     "fb_last_error": (C.c_char_p, []),

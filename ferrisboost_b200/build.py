@@ -18,7 +18,8 @@ HERE = pathlib.Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libfbgpu.so"
 SOURCES = ["train_kernels.cu", "explain_kernels.cu", "ctx.cu", "engine.cu", "noalloc.cu", "nccl_loader.cu", "lossguide.cu",
-           "sketch.cu", "shap_paths.cu", "hist_ceiling.cu", "qscale.cu", "devmem.cu"]
+           "sketch.cu", "shap_paths.cu", "hist_ceiling.cu", "qscale.cu", "devmem.cu",
+           "embed.cu", "dropout.cu", "sample.cu"]
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
 
 

@@ -1,0 +1,228 @@
+"""Operators on a model's leaves and class scores, on tensors in GPU memory.
+
+A trained model gives each row's leaf in every tree (``predict(pred_leaf=True)``)
+and, for multiclass objectives, a score for each class.  ``embed`` looks up and
+sums a vector for each leaf (or categorical code), ``embed_grad`` is its
+gradient for the table, ``dropout`` drops elements by a seed and their index,
+and ``sample`` draws a class from a row of scores.
+
+The functions take torch CUDA tensors (float32, float16 or bfloat16) and return
+new ones, or fill ``out``.  Like torch's own operations they are enqueued on the
+current stream of the tensors' device and do not wait for it; a tensor made on
+another stream needs the usual ``wait_stream`` / ``record_stream``.  They can be
+captured into a CUDA graph.  Wrong arguments raise ValueError before anything
+is enqueued.  The kernels are ``fbgpu_embed``, ``fbgpu_embed_grad``,
+``fbgpu_dropout`` and ``fbgpu_sample`` of include/fbgpu.h, which has the exact
+definitions; there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Any
+
+import torch
+
+from . import _lib
+
+__all__ = ["embed", "embed_grad", "dropout", "sample"]
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # FBGPU_F32, FBGPU_F16, FBGPU_BF16
+_TOKENS = {torch.int32: 0, torch.int64: 1}                        # FBGPU_I32, FBGPU_I64
+
+
+def _type(name: str, t: Any, dims: int | None, types: dict) -> int:
+    """The type code of a CUDA tensor, with its dimensions checked."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device, it is on {t.device}")
+    if dims is not None and t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimension(s), got shape {tuple(t.shape)}")
+    code = types.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be one of {', '.join(str(k) for k in types)}, got {t.dtype}")
+    return code
+
+
+def _rows(name: str, t: torch.Tensor) -> int:
+    """The row stride of a 2-D tensor whose rows are contiguous."""
+    row, col = t.stride()
+    if col != 1 and t.shape[1] > 1:
+        raise ValueError(f"{name} must have contiguous rows, its strides are {(row, col)}")
+    return row
+
+
+def _same_device(t: torch.Tensor, **others: Any) -> None:
+    device = t.get_device()
+    for name, o in others.items():
+        if o is not None and o.get_device() != device:
+            raise ValueError(f"{name} is on cuda:{o.get_device()}, the other tensors are on cuda:{device}")
+
+
+def _out(out: Any, shape: tuple, like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != like.dtype:
+        raise ValueError(f"out must be a {like.dtype} tensor of shape {shape}")
+    _same_device(like, out=out)
+    return out
+
+
+def _call(t: torch.Tensor, fn: str, *args: Any) -> None:
+    """Calls the entry point on t's device, with that device's current stream as the last argument."""
+    device = t.get_device()
+    f = getattr(_lib.load(), fn)
+    if device == torch.cuda.current_device():
+        status = f(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = f(*args, torch.cuda.current_stream(device).cuda_stream)
+    if status:
+        message = (_lib.load().fbgpu_last_error(None) or b"").decode()
+        raise (ValueError if status == 1 else RuntimeError)(message)
+
+
+def _token_shape(tokens: torch.Tensor) -> tuple:
+    """(token code, rows, tokens per row, row stride, column stride)"""
+    code = _type("tokens", tokens, None, _TOKENS)
+    if tokens.dim() == 1:
+        return code, tokens.shape[0], 1, tokens.stride(0), 1
+    if tokens.dim() == 2:
+        return code, tokens.shape[0], tokens.shape[1], tokens.stride(0), tokens.stride(1)
+    raise ValueError(f"tokens must have 1 or 2 dimensions, got shape {tuple(tokens.shape)}")
+
+
+def _count(dim: int, k: int) -> None:
+    """The entry points take 32-bit row lengths."""
+    if dim >= 1 << 32 or k >= 1 << 32:
+        raise ValueError(f"rows of {dim} elements and {k} tokens: both must be below 2**32")
+
+
+def embed(table: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0,
+          out: torch.Tensor | None = None) -> torch.Tensor:
+    """``scale`` times the sum of the table rows that each row's tokens name.
+
+    ``table`` is vocab x dim; ``tokens`` (int32 or int64, any strides) is n, or
+    n x k for k tokens a row, such as a row's leaf in each of k trees with the
+    tree's first node added.  A token outside [0, vocab) stands for a missing
+    value and adds nothing.  The sum is taken in float32 and rounded once.
+    Returns n x dim in the table's type."""
+    code = _type("table", table, 2, _TYPES)
+    tcode, n, k, trow, tcol = _token_shape(tokens)
+    _same_device(table, tokens=tokens)
+    vocab, dim = table.shape
+    _count(dim, k)
+    out = _out(out, (n, dim), table)
+    _call(table, "fbgpu_embed", table.data_ptr(), code, vocab, dim, _rows("table", table), tokens.data_ptr(), tcode, n,
+          k, trow, tcol, scale, out.data_ptr(), _rows("out", out))
+    return out
+
+
+def embed_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale: float = 1.0,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of ``embed`` for its table, vocab x dim in grad's type.
+
+    ``grad`` (n x dim) is the gradient of ``embed``'s result for the same
+    ``tokens`` and ``scale``.  Row v is ``scale`` times the float32 sum of
+    grad[r] over the places (r, j) with token v, zero where there is none.
+    The same inputs give the same bits: the places are sorted by token and no
+    atomic adds are used.  n * k and vocab are at most 2**31 - 2."""
+    code = _type("grad", grad, 2, _TYPES)
+    tcode, n, k, trow, tcol = _token_shape(tokens)
+    _same_device(grad, tokens=tokens)
+    vocab = int(vocab)
+    if vocab < 0:
+        raise ValueError(f"vocab must not be negative, got {vocab}")
+    if grad.shape[0] != n:
+        raise ValueError(f"grad has {grad.shape[0]} rows, tokens has {n}")
+    dim = grad.shape[1]
+    _count(dim, k)
+    out = _out(out, (vocab, dim), grad)
+    size = _lib.load().fbgpu_embed_grad_workspace(n, k, vocab, dim)
+    space = torch.empty(size, dtype=torch.uint8, device=grad.device)
+    _call(grad, "fbgpu_embed_grad", grad.data_ptr(), code, n, k, dim, _rows("grad", grad), tokens.data_ptr(), tcode,
+          trow, tcol, vocab, scale, out.data_ptr(), _rows("out", out), space.data_ptr(), size)
+    return out
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, *,
+            out: torch.Tensor | None = None) -> torch.Tensor:
+    """x / (1 - p) where an element is kept, else 0.
+
+    Whether element i (in row-major order) is kept follows from ``seed`` and
+    ``offset + i`` alone, not from x's strides, so no mask is stored:
+    ``dropout(grad, p, seed, offset)`` is the backward pass.  Steps that must
+    differ take another seed, or an offset that is further by the number of
+    elements.  ``x`` has any shape if it is contiguous, else two dimensions with
+    contiguous rows.  ``out=x`` works in place."""
+    code = _type("x", x, None, _TYPES)
+    p = float(p)
+    out = _out(out, tuple(x.shape), x)
+    if x.is_contiguous() and out.is_contiguous():
+        n, dim = 1, x.numel()
+        xs = os = dim
+    elif x.dim() == 2:
+        n, dim = x.shape
+        xs, os = _rows("x", x), _rows("out", out)
+    else:
+        raise ValueError(f"x and out must be contiguous, or 2-D with contiguous rows; x has shape {tuple(x.shape)} "
+                         f"and strides {x.stride()}")
+    _call(x, "fbgpu_dropout", x.data_ptr(), code, n, dim, xs, p, seed & 0xFFFFFFFFFFFFFFFF,
+          offset & 0xFFFFFFFFFFFFFFFF, out.data_ptr(), os)
+    return out
+
+
+def _limit(name: str, value: Any, scores: torch.Tensor, dtype: torch.dtype) -> tuple:
+    """(scalar, pointer) of a limit given as a number or as a tensor with a value for each row."""
+    if not isinstance(value, torch.Tensor):
+        return value, None
+    if value.dtype != dtype or value.shape != scores.shape[:1] or not value.is_contiguous():
+        raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {scores.shape[0]} values")
+    _same_device(scores, **{name: value})
+    return 0, value.data_ptr()
+
+
+def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: Any = 1.0, top_k: Any = 0, top_p: Any = 1.0,
+           min_p: Any = 0.0, classes: torch.Tensor | None = None,
+           probs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Draws a class from each row of scores; returns (classes, probs).
+
+    ``scores`` is n x K (2 <= K <= 2**20): margins or logits, in which -inf and
+    NaN rule a class out.  ``u`` has a float32 random number in [0, 1) for each
+    row.  The softmax of scores / ``temperature`` is limited to the ``top_k``
+    largest (0: no limit), then to the shortest beginning of the falling order
+    that holds ``top_p`` of their total, then to classes at least ``min_p``
+    times as probable as the first; equal scores are ordered by class.  The
+    class drawn (int32) is the first, by class, at which the running sum of
+    what is left passes u times its total, and ``probs`` (float32) is its share.
+    ``temperature`` 0 gives the first maximum.  A row with every class ruled out
+    gives class -1 and share 0.  Each limit is a number or a tensor with a
+    value for each row (float32; ``top_k`` int32).  Weights are whole multiples
+    of 2**-40 of the first class's, so a draw does not depend on the order of
+    sums; classes below that are never drawn."""
+    code = _type("scores", scores, 2, _TYPES)
+    n, k = scores.shape
+    _type("u", u, 1, {torch.float32: 0})
+    if u.shape[0] != n or not u.is_contiguous():
+        raise ValueError(f"u must be contiguous with {n} values, got shape {tuple(u.shape)}")
+    _same_device(scores, u=u)
+    t, ts = _limit("temperature", temperature, scores, torch.float32)
+    tk, tks = _limit("top_k", top_k, scores, torch.int32)
+    tp, tps = _limit("top_p", top_p, scores, torch.float32)
+    mp, mps = _limit("min_p", min_p, scores, torch.float32)
+    if tks is None and (tk != int(tk) or not 0 <= tk < 1 << 31):
+        raise ValueError(f"top_k must be a whole number in 0..2**31 - 1, got {tk}")
+    if k > 1 << 20:
+        raise ValueError(f"classes must be in 2..1048576, got {k}")
+    if classes is None:
+        classes = torch.empty(n, dtype=torch.int32, device=scores.device)
+    if probs is None:
+        probs = torch.empty(n, dtype=torch.float32, device=scores.device)
+    for name, t_, dtype in (("classes", classes, torch.int32), ("probs", probs, torch.float32)):
+        if t_.dtype != dtype or t_.shape != u.shape or not t_.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values")
+        _same_device(scores, **{name: t_})
+    params = _lib.FbgpuSampleParams(t, int(tk), tp, mp, ts, tks, tps, mps)
+    _call(scores, "fbgpu_sample", scores.data_ptr(), code, n, k, _rows("scores", scores), u.data_ptr(),
+          C.byref(params), classes.data_ptr(), probs.data_ptr())
+    return classes, probs

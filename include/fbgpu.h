@@ -420,6 +420,94 @@ fbgpu_status fbgpu_explain(fbgpu_model* m, int32_t kind, const float* X, uint64_
 fbgpu_status fbgpu_explain_device(fbgpu_model* m, int32_t kind, const float* X, uint64_t n, float* out,
                                   void* stream);
 
+/* ---------------------------------------------- leaf vectors and class draws
+ *
+ * Operators on what a model hands on: the tokens that fbgpu_explain's leaf
+ * indices (or categorical codes) make, and the class scores.  No counterpart in
+ * the reference.  Every array is a device pointer of the current device and
+ * work is enqueued on `stream` (a cudaStream_t of that device, NULL = default
+ * stream); nothing is allocated and nothing waits, so the calls can be captured
+ * into a graph.  A matrix is rows of contiguous elements; its stride is the
+ * elements from one row to the next.  Arrays are aligned to their element.
+ * Sizes and pointers are checked before anything is enqueued (FBGPU_EINPUT);
+ * the messages are in fbgpu_last_error(NULL).  Outputs must not overlap inputs
+ * unless a call says so. */
+
+/* Element types, and token types. */
+#define FBGPU_F32 0
+#define FBGPU_F16 1
+#define FBGPU_BF16 2
+#define FBGPU_I32 0
+#define FBGPU_I64 1
+
+/* out[r] = scale * sum over j < per_row of table[token(r, j)], r < n: rows of
+ * `dim` elements of `type`, summed in f32 and rounded once.  Token (r, j) is at
+ * tokens + r * token_row + j * token_col; one outside [0, vocab) stands for a
+ * missing value and adds nothing (a row of only such tokens is zero).  The
+ * order of the sum depends on the sizes alone. */
+fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vocab, uint32_t dim, uint64_t table_stride,
+                         const void* tokens, int32_t token_type, uint64_t n, uint32_t per_row, uint64_t token_row,
+                         uint64_t token_col, float scale, void* out, uint64_t out_stride, void* stream);
+
+/* The gradient of fbgpu_embed for its table: out[v] = scale * sum of grad[r]
+ * over the places (r, j) that hold token v, vocab rows of `dim` elements,
+ * every one written.  The places are sorted by token (stable), so that each
+ * row is summed in f32 in an order that depends on the tokens alone, with no
+ * atomics: the same inputs give the same bits.  grad's stride may be 0 (one row
+ * for all).  n * per_row and vocab are at most 2^31 - 2.  `workspace` holds
+ * fbgpu_embed_grad_workspace(...) bytes, 256-byte aligned, with any contents. */
+uint64_t fbgpu_embed_grad_workspace(uint64_t n, uint32_t per_row, uint64_t vocab, uint32_t dim);
+fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_t n, uint32_t per_row, uint32_t dim,
+                              uint64_t grad_stride, const void* tokens, int32_t token_type, uint64_t token_row,
+                              uint64_t token_col, uint64_t vocab, float scale, void* out, uint64_t out_stride,
+                              void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* out = x / (1 - p) where an element is kept, else 0 (whatever x is there).
+ * Element (r, c) of the n x dim matrix has the number e = offset + r * dim + c
+ * and the 32 random bits of half e % 2 (0 = low) of word e / 2 of a SplitMix64
+ * sequence (Steele, Lea and Flood 2014): word w is mix(mix(seed) + (w + 1) *
+ * 0x9E3779B97F4A7C15), mix being that generator's finalizer, the one that row
+ * sampling uses.  It is kept when they are at least ceil(p * 2^32), 0 <= p <= 1.
+ * So the mask is never stored, does not depend on strides, and the call on
+ * the gradient with the same p, seed and offset is the backward pass.  out may
+ * be x itself (same pointer and stride). */
+fbgpu_status fbgpu_dropout(const void* x, int32_t type, uint64_t n, uint64_t dim, uint64_t x_stride, double p,
+                           uint64_t seed, uint64_t offset, void* out, uint64_t out_stride, void* stream);
+
+/* Limits of a draw: one value for all rows, or, where the array is not NULL, a
+ * value for each row (f32, top_k int32).  temperature 0 draws the first
+ * maximum.  top_k 0, top_p 1 and min_p 0 are no limit.  Values of an array
+ * outside the ranges are read so: a temperature that is not above 0 as 0, a top_k
+ * below 1 as none, top_p below 0 as 0 and NaN as 1, min_p above 1 as 1 and NaN
+ * as 0. */
+typedef struct fbgpu_sample_params {
+    float temperature;  /* >= 0 */
+    int32_t top_k;      /* >= 0 */
+    float top_p;        /* 0..1 */
+    float min_p;        /* 0..1 */
+    const float* temperatures;
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+} fbgpu_sample_params;
+
+/* Draws a class for each of n rows of `classes` scores x (2..2^20 of them).  A
+ * class weighs w = floor(2^40 exp((x - max) / temperature)) (exp in f32; a score
+ * of -infinity or NaN weighs 0; where the maximum is +infinity, its classes
+ * weigh 2^40 and the others 0).  In the order of falling scores, equal ones by
+ * class: top_k keeps the first top_k classes; of their total S, top_p then
+ * keeps the shortest beginning of at least ceil(top_p * S), one class at
+ * least; min_p then keeps the classes whose exp is at least min_p.  With S the
+ * total of what is left and u[r] in [0, 1) the row's random number, the class
+ * drawn is the first, by class, at which the sum of the kept weights is above
+ * floor(u * S).  The sums are whole numbers, so the draw does not depend on how
+ * the work is split.  out_classes[r] gets the class (-1 where every score is
+ * -infinity or NaN) and out_probs[r], unless NULL, its share w / S of the kept
+ * weight (0 for -1). */
+fbgpu_status fbgpu_sample(const void* scores, int32_t type, uint64_t n, uint32_t classes, uint64_t stride,
+                          const float* u, const fbgpu_sample_params* params, int32_t* out_classes, float* out_probs,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif
