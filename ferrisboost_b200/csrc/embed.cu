@@ -6,8 +6,13 @@
 //
 // The gradient sorts the places by token with a stable radix sort (least
 // significant digit first) whose payload is the place's row, so that a token's
-// rows are consecutive and in ascending order; each table row is then one
-// sum over a run of the sorted list, with no atomics.
+// rows are consecutive and in ascending order, and then sums the sorted list in
+// equal parts, whatever the lengths of the tokens' runs.  A run inside a part is
+// written at once; what continues into another part is joined from the parts'
+// sums in a second pass.  No atomics: the order of every sum follows from the
+// tokens and the sizes.
+#include <cooperative_groups.h>
+
 #include "ops.h"
 
 namespace fbg {
@@ -206,40 +211,276 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_scatter(SortPass a, Token
     }
 }
 
+// A sort of up to CTAS * 8192 places in one launch: the blocks of one cluster
+// hold the places, read one another's digit counts and exchange places through
+// the (L2-resident) buffers.  The remaining blocks of the grid clear the output.
+constexpr int kClusterThreads = 512, kClusterItems = 16, kClusterTile = kClusterThreads * kClusterItems;
+
+struct Clear {
+    char* p;          // rows of `bytes` bytes, `stride` bytes apart
+    uint64_t rows, bytes, stride;
+};
+
+// Block `b` of `blocks` clears its share.
+__device__ __forceinline__ void clear_rows(const Clear& z, uint64_t b, uint64_t blocks) {
+    const uint64_t per = 16ull * blockDim.x;  // bytes of a block's step
+    const uint64_t steps = (z.bytes + 15 + per - 1) / per;
+    for (uint64_t i = b; i < z.rows * steps; i += blocks) {
+        const uint64_t r = z.rows == 1 ? 0 : i / steps;
+        char* row = z.p + r * z.stride;
+        char* end = row + z.bytes;
+        char* at = reinterpret_cast<char*>((uintptr_t)row & ~(uintptr_t)15) + (i - r * steps) * per + 16 * threadIdx.x;
+        if (at >= row && at + 16 <= end) {
+            *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+        } else {  // elements are two or four bytes
+            for (int k = 0; k < 16; k += 2)
+                if (at + k >= row && at + k < end) *reinterpret_cast<uint16_t*>(at + k) = 0;
+        }
+    }
+}
+__global__ void __launch_bounds__(256) k_clear(Clear z) { clear_rows(z, blockIdx.x, gridDim.x); }
+
+struct ClusterSort {
+    uint32_t *keys[2], *rows[2];  // pass p writes set p & 1
+    uint32_t count, bits, passes;
+};
+
+template <class Tok, int CTAS>
+__global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(ClusterSort a, Tokens<Tok> tokens, uint32_t per_row,
+                                                                  uint64_t vocab, Clear z) {
+    if (blockIdx.x >= CTAS) {
+        clear_rows(z, blockIdx.x - CTAS, gridDim.x - CTAS);
+        return;
+    }
+    constexpr int kWarps = kClusterThreads / 32;
+    __shared__ uint16_t seen[kWarps][kMaxBins];
+    __shared__ uint32_t total[kMaxBins], dest[kMaxBins], part[kWarps];
+    const auto cluster = cooperative_groups::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = CTAS == 1 ? 0 : cluster.block_rank();
+    const uint32_t bins = 1u << a.bits, base = cta * kClusterTile + warp * (kClusterTile / kWarps) + lane;
+    for (uint32_t pass = 0; pass < a.passes; pass++) {
+        const uint32_t shift = pass * a.bits;
+        for (uint32_t b = threadIdx.x; b < kWarps * kMaxBins; b += kClusterThreads) (&seen[0][0])[b] = 0;
+        uint32_t key[kClusterItems], row[kClusterItems], rank[kClusterItems];
+#pragma unroll
+        for (int k = 0; k < kClusterItems; k++) {
+            const uint32_t i = base + k * 32;
+            key[k] = row[k] = 0;
+            if (i >= a.count) continue;
+            if (pass == 0) {
+                row[k] = i / per_row;
+                key[k] = (uint32_t)tokens.at(row[k], i - row[k] * per_row, vocab);
+            } else {
+                key[k] = __ldcg(a.keys[(pass - 1) & 1] + i);
+                row[k] = __ldcg(a.rows[(pass - 1) & 1] + i);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kClusterItems; k++) {
+            const bool in = base + k * 32 < a.count;
+            const uint32_t d = in ? (key[k] >> shift) & (bins - 1) : kMaxBins;
+            const uint32_t peers = __match_any_sync(0xffffffffu, d);
+            const int lead = __ffs(peers) - 1;
+            uint32_t old = 0;
+            if (in && lane == lead) {
+                old = seen[warp][d];
+                seen[warp][d] = (uint16_t)(old + __popc(peers));
+            }
+            __syncwarp();
+            rank[k] = __shfl_sync(0xffffffffu, old, lead) + __popc(peers & ((1u << lane) - 1));
+        }
+        __syncthreads();
+        const uint32_t d = threadIdx.x;  // kMaxBins is the number of threads
+        uint32_t mine = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const uint32_t c = seen[w][d];
+            seen[w][d] = (uint16_t)mine;
+            mine += c;
+        }
+        total[d] = mine;
+        if (CTAS > 1) cluster.sync();
+        uint32_t all = 0, before = 0;
+#pragma unroll
+        for (int c = 0; c < CTAS; c++) {
+            const uint32_t t = CTAS == 1 ? mine : cluster.map_shared_rank(total, c)[d];
+            all += t;
+            if (c < cta) before += t;
+        }
+        uint32_t sum;
+        dest[d] = before + block_scan<kClusterThreads>(all, part, sum);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kClusterItems; k++) {
+            if (base + k * 32 < a.count) {
+                const uint32_t dk = (key[k] >> shift) & (bins - 1);
+                const uint32_t to = dest[dk] + seen[warp][dk] + rank[k];
+                a.keys[pass & 1][to] = key[k];
+                a.rows[pass & 1][to] = row[k];
+            }
+        }
+        // the places' order is read by every block, and `total` is no longer read
+        if (CTAS > 1) cluster.sync();
+        else __syncthreads();
+    }
+}
+static_assert(kMaxBins == kClusterThreads, "a thread per bin");
+
 // ------------------------------------------------------------- run sums
-// Where each token's run of the sorted places begins and ends (both zero from
-// before for a token with none).
-__global__ void k_runs(const uint32_t* __restrict__ keys, uint32_t count, uint32_t vocab, uint32_t* __restrict__ begin,
-                       uint32_t* __restrict__ end) {
-    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= count) return;
-    const uint32_t k = keys[i];
-    if (k >= vocab) return;
-    if (i == 0 || keys[i - 1] != k) begin[k] = i;
-    if (i + 1 == count || keys[i + 1] != k) end[k] = i + 1;
+// A group of `lanes` threads sums `chunk` consecutive places of the sorted list
+// (a slice of V * lanes columns of their rows), eight loads in flight.  Its first
+// run may continue from the group before (its "head") and its last into the
+// next (its "tail"); the others are complete and written.  Then each group
+// with a tail that began in it adds the heads of the groups that the run
+// goes on through.  What leaves the block is kept in `part`: [block][0] the sum
+// of the run that came in, [block][1] of the one that goes out.
+constexpr int kRunThreads = 256, kAhead = 8;
+constexpr uint32_t kMostChunk = 64, kFewBlocks = 148 * 4, kMostSlices = 65535;
+
+struct RunSums {
+    const uint32_t *keys, *rows;
+    float* part;
+    uint32_t count, vocab, dim, lanes, chunk;
+    uint64_t grad_stride, out_stride;
+    float scale;
+};
+
+__device__ __forceinline__ uint32_t key_at(const RunSums& a, uint64_t i) { return i < a.count ? a.keys[i] : a.vocab; }
+
+template <class T, int V> __device__ __forceinline__ void write_row(const RunSums& a, T* out, uint32_t key, uint32_t c,
+                                                                    const float* acc) {
+    Pack<T, V> o;
+#pragma unroll
+    for (int k = 0; k < V; k++) o.v[k] = from_f32<T>(acc[k] * a.scale);
+    *reinterpret_cast<Pack<T, V>*>(out + key * a.out_stride + c) = o;
 }
 
-// A group of lanes makes one row of the gradient.
 template <class T, int V>
-__global__ void __launch_bounds__(256) k_run_sums(const T* __restrict__ grad, uint32_t dim, uint64_t grad_stride,
-                                                  const uint32_t* __restrict__ rows, const uint32_t* __restrict__ begin,
-                                                  const uint32_t* __restrict__ end, uint32_t vocab, float scale,
-                                                  T* __restrict__ out, uint64_t out_stride, uint32_t lanes) {
-    const uint32_t lane = threadIdx.x & (lanes - 1);
-    const uint64_t v = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) / lanes;
-    if (v >= vocab) return;
-    const uint32_t b = begin[v], e = end[v];
-    for (uint32_t c = lane * V; c < dim; c += lanes * V) {
-        float acc[V] = {};
-        for (uint32_t i = b; i < e; i++) {
-            const Pack<T, V> g = *reinterpret_cast<const Pack<T, V>*>(grad + rows[i] * grad_stride + c);
+__global__ void __launch_bounds__(kRunThreads) k_run_sums(RunSums a, const T* __restrict__ grad, T* __restrict__ out) {
+    __shared__ float heads[kRunThreads * V];  // [group][V * lanes]
+    __shared__ uint8_t goes_on[kRunThreads];  // the group is one run, from before its first place to after its last
+    const uint32_t groups = kRunThreads / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x & (a.lanes - 1);
+    const uint32_t c = (blockIdx.y * a.lanes + lane) * V;
+    const bool column = c < a.dim;
+    const uint64_t begin = ((uint64_t)blockIdx.x * groups + group) * a.chunk;
+    uint32_t cur = key_at(a, begin);
+    const bool from_before = begin > 0 && cur < a.vocab && key_at(a, begin - 1) == cur;
+    bool head = from_before;  // the current run is the one that came in
+    float acc[V] = {};
+    for (uint32_t p = 0; p < a.chunk; p += kAhead) {
+        uint32_t key[kAhead], row[kAhead];
+        Pack<T, V> g[kAhead];
 #pragma unroll
-            for (int k = 0; k < V; k++) acc[k] += to_f32(g.v[k]);
+        for (int k = 0; k < kAhead; k++) {
+            key[k] = key_at(a, begin + p + k);
+            row[k] = key[k] < a.vocab ? a.rows[begin + p + k] : 0;
         }
-        Pack<T, V> o;
 #pragma unroll
-        for (int k = 0; k < V; k++) o.v[k] = from_f32<T>(acc[k] * scale);
-        *reinterpret_cast<Pack<T, V>*>(out + v * out_stride + c) = o;
+        for (int k = 0; k < kAhead; k++)
+            if (column && key[k] < a.vocab)
+                g[k] = *reinterpret_cast<const Pack<T, V>*>(grad + row[k] * a.grad_stride + c);
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            if (key[k] != cur) {
+                if (head) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc[i];
+                } else if (column) {
+                    write_row<T, V>(a, out, cur, c, acc);
+                }
+                head = false;
+                cur = key[k];
+#pragma unroll
+                for (int i = 0; i < V; i++) acc[i] = 0.0f;
+            }
+            if (column && key[k] < a.vocab) {
+#pragma unroll
+                for (int i = 0; i < V; i++) acc[i] += to_f32(g[k].v[i]);
+            }
+        }
+    }
+    const bool to_after = cur < a.vocab && key_at(a, begin + a.chunk) == cur;
+    if (head) {
+#pragma unroll
+        for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc[i];
+    } else if (!to_after && cur < a.vocab && column) {
+        write_row<T, V>(a, out, cur, c, acc);
+    }
+    if (lane == 0) goes_on[group] = head && to_after;
+    __syncthreads();
+    const uint64_t block = (uint64_t)blockIdx.x * 2 * a.dim;
+    if (!head && to_after) {  // a run that began here
+        uint32_t h = group + 1;
+        bool open = true;
+        for (; h < groups && open; h++) {
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] += heads[(h * a.lanes + lane) * V + i];
+            open = goes_on[h];
+        }
+        if (column) {
+            if (open) {
+#pragma unroll
+                for (int i = 0; i < V; i++) a.part[block + a.dim + c + i] = acc[i];
+            } else {
+                write_row<T, V>(a, out, cur, c, acc);
+            }
+        }
+    }
+    if (group == 0 && from_before && column) {  // the run that came into the block
+        float sum[V] = {};
+        bool open = true;
+        for (uint32_t h = 0; h < groups && open; h++) {
+#pragma unroll
+            for (int i = 0; i < V; i++) sum[i] += heads[(h * a.lanes + lane) * V + i];
+            open = goes_on[h];
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) a.part[block + c + i] = sum[i];
+    }
+}
+
+// A block joins the run that leaves block x of k_run_sums, if it began there:
+// its own part and what the following blocks it goes through (and the one it
+// ends in) have of it, each group a share of the blocks, then the groups.
+template <class T, int V>
+__global__ void __launch_bounds__(kRunThreads) k_run_joins(RunSums a, T* __restrict__ out) {
+    __shared__ float sums[kRunThreads * V];
+    const uint32_t groups = kRunThreads / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x & (a.lanes - 1);
+    const uint64_t span = (uint64_t)groups * a.chunk, begin = blockIdx.x * span, end = begin + span;
+    const uint32_t key = key_at(a, end - 1);
+    if (key >= a.vocab || key_at(a, end) != key) return;                            // no run leaves
+    if (begin > 0 && key_at(a, begin - 1) == key) return;                           // it only goes through
+    uint32_t more = 0;  // the following blocks that start in the run
+    for (uint32_t b = 1;; b += kRunThreads) {
+        const uint32_t here = __syncthreads_count(key_at(a, begin + (b + threadIdx.x) * span) == key);
+        more += here;
+        if (here < kRunThreads) break;
+    }
+    const uint32_t c = (blockIdx.y * a.lanes + lane) * V;
+    const bool column = c < a.dim;
+    float acc[V] = {};
+    if (column) {
+        const float* part = a.part + (uint64_t)blockIdx.x * 2 * a.dim + c;
+        if (group == 0) {
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] = part[a.dim + i];
+        }
+#pragma unroll 4
+        for (uint32_t b = 1 + group; b <= more; b += groups) {
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] += part[(uint64_t)b * 2 * a.dim + i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) sums[threadIdx.x * V + i] = acc[i];
+    __syncthreads();
+    if (group == 0 && column) {
+        for (uint32_t h = 1; h < groups && h <= more; h++) {
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] += sums[(h * a.lanes + lane) * V + i];
+        }
+        write_row<T, V>(a, out, key, c, acc);
     }
 }
 
@@ -279,9 +520,9 @@ uint64_t token_extent(uint64_t n, uint64_t per_row, uint64_t row, uint64_t col, 
 
 // Parts of the gradient's workspace, each 256-byte aligned.
 struct GradSpace {
-    uint64_t keys[2], rows[2], hist, total, begin, end, bytes;
+    uint64_t keys[2], rows[2], hist, total, part, bytes;
     uint32_t count, tiles, bits, passes;
-    GradSpace(uint64_t n, uint64_t per_row, uint64_t vocab) {
+    GradSpace(uint64_t n, uint64_t per_row, uint64_t vocab, uint32_t dim) {
         count = (uint32_t)(n * per_row);
         tiles = ceil_div(count, kTile);
         bits = 1;
@@ -297,8 +538,10 @@ struct GradSpace {
         for (int i = 0; i < 2; i++) keys[i] = take(4ull * count), rows[i] = take(4ull * count);
         hist = take(4ull * (1ull << bits) * tiles);
         total = take(4ull << bits);
-        begin = take(8ull * vocab);
-        end = begin + 4 * vocab;
+        // two rows for each block of k_run_sums; a chunk below the longest is only taken for few blocks
+        const uint32_t groups = kRunThreads / lanes_for(dim);  // the fewest of any vector width
+        part = take(8ull * dim * std::min(ceil_div(count, groups * kAhead),
+                                          std::max(ceil_div(count, groups * kMostChunk), 2 * kFewBlocks)));
         bytes = at;
     }
 };
@@ -350,8 +593,7 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
 }
 
 extern "C" uint64_t fbgpu_embed_grad_workspace(uint64_t n, uint32_t per_row, uint64_t vocab, uint32_t dim) {
-    (void)dim;
-    return fbg::grad_sizes_fit(n, per_row, vocab) ? fbg::GradSpace(n, per_row, vocab).bytes : 0;
+    return fbg::grad_sizes_fit(n, per_row, vocab) ? fbg::GradSpace(n, per_row, vocab, dim).bytes : 0;
 }
 
 extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_t n, uint32_t per_row, uint32_t dim,
@@ -366,10 +608,11 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
         check_matrix("out", out, vocab, dim, out_stride, size, true);
         if (!grad_sizes_fit(n, per_row, vocab))
             throw InputError("fbgpu_embed_grad takes at most 2147483646 places and as many tokens");
+        if (dim > kMostSlices * 32) throw InputError("fbgpu_embed_grad takes rows of at most 2097120 elements");
         with_token(token_type, [&](auto tok) {
             using Tok = decltype(tok);
             check_tokens(tokens, n, per_row, token_row, token_col, sizeof(Tok));
-            const GradSpace ws(n, per_row, vocab);
+            const GradSpace ws(n, per_row, vocab, dim);
             if (workspace_bytes < ws.bytes || (!workspace && ws.bytes))
                 throw InputError("the workspace is smaller than fbgpu_embed_grad_workspace says");
             if ((uintptr_t)workspace % 256) throw InputError("the workspace must be 256-byte aligned");
@@ -384,47 +627,97 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
             if (!vocab || !dim) return;
             char* w = static_cast<char*>(workspace);
             auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
-            FB_CUDA_CHECK(cudaMemsetAsync(w + ws.begin, 0, 8 * vocab, s));
             const Tokens<Tok> tk{static_cast<const Tok*>(tokens), token_row, token_col};
-            for (uint32_t p = 0; ws.count && p < ws.passes; p++) {
-                SortPass a{};
-                a.keys = p ? at(ws.keys[(p - 1) & 1]) : nullptr;
-                a.rows = p ? at(ws.rows[(p - 1) & 1]) : nullptr;
-                a.keys_out = at(ws.keys[p & 1]);
-                a.rows_out = at(ws.rows[p & 1]);
-                a.hist = at(ws.hist);
-                a.total = at(ws.total);
-                a.count = ws.count;
-                a.tiles = ws.tiles;
-                a.shift = p * ws.bits;
-                a.bins = 1u << ws.bits;
-                for (int k = 0; k < 3; k++) count_launch();
-                if (p == 0) {
-                    k_sort_count<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
-                    k_sort_scan<<<a.bins, kSortThreads, 0, s>>>(a);
-                    k_sort_scatter<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
-                } else {
-                    k_sort_count<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
-                    k_sort_scan<<<a.bins, kSortThreads, 0, s>>>(a);
-                    k_sort_scatter<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
+            Clear z{static_cast<char*>(out), vocab, (uint64_t)dim * size, out_stride * size};
+            if (out_stride == dim) z = Clear{z.p, 1, vocab * z.bytes, 0};
+            const uint64_t cleared = z.rows * ((z.bytes + 15) / 16);
+            if (ws.count == 0 || ws.count > 8 * kClusterTile) {
+                count_launch();
+                k_clear<<<(uint32_t)std::min<uint64_t>(148 * 8, (cleared + 255) / 256), 256, 0, s>>>(z);
+            }
+            if (ws.count == 0) {
+                FB_CUDA_CHECK(cudaGetLastError());
+                return;
+            }
+            if (ws.count <= 8 * kClusterTile) {
+                ClusterSort a{{at(ws.keys[0]), at(ws.keys[1])}, {at(ws.rows[0]), at(ws.rows[1])}, ws.count, ws.bits,
+                              ws.passes};
+                auto launch = [&](auto ctas) {
+                    constexpr int kCtas = decltype(ctas)::value;
+                    const uint64_t wish = (cleared + 4 * kClusterThreads - 1) / (4 * kClusterThreads);
+                    cudaLaunchConfig_t cfg{};
+                    cfg.gridDim = dim3(kCtas + ((uint32_t)std::min<uint64_t>(148 * 3, wish) + kCtas - 1) / kCtas * kCtas);
+                    cfg.blockDim = dim3(kClusterThreads);
+                    cfg.stream = s;
+                    cudaLaunchAttribute attr{};
+                    attr.id = cudaLaunchAttributeClusterDimension;
+                    attr.val.clusterDim.x = kCtas;
+                    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+                    cfg.attrs = &attr;
+                    cfg.numAttrs = kCtas > 1 ? 1 : 0;
+                    count_launch();
+                    FB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sort_cluster<Tok, kCtas>, a, tk, per_row, vocab, z));
+                };
+                const uint32_t need = ceil_div(ws.count, kClusterTile);
+                if (need == 1) launch(std::integral_constant<int, 1>{});
+                else if (need == 2) launch(std::integral_constant<int, 2>{});
+                else if (need <= 4) launch(std::integral_constant<int, 4>{});
+                else launch(std::integral_constant<int, 8>{});
+            } else {
+                for (uint32_t p = 0; p < ws.passes; p++) {
+                    SortPass a{};
+                    a.keys = p ? at(ws.keys[(p - 1) & 1]) : nullptr;
+                    a.rows = p ? at(ws.rows[(p - 1) & 1]) : nullptr;
+                    a.keys_out = at(ws.keys[p & 1]);
+                    a.rows_out = at(ws.rows[p & 1]);
+                    a.hist = at(ws.hist);
+                    a.total = at(ws.total);
+                    a.count = ws.count;
+                    a.tiles = ws.tiles;
+                    a.shift = p * ws.bits;
+                    a.bins = 1u << ws.bits;
+                    for (int k = 0; k < 3; k++) count_launch();
+                    if (p == 0) {
+                        k_sort_count<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
+                        k_sort_scan<<<a.bins, kSortThreads, 0, s>>>(a);
+                        k_sort_scatter<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
+                    } else {
+                        k_sort_count<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
+                        k_sort_scan<<<a.bins, kSortThreads, 0, s>>>(a);
+                        k_sort_scatter<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
+                    }
                 }
             }
             const int last = (ws.passes - 1) & 1;
-            if (ws.count) {
-                count_launch();
-                k_runs<<<ceil_div(ws.count, 256), 256, 0, s>>>(at(ws.keys[last]), ws.count, (uint32_t)vocab,
-                                                               at(ws.begin), at(ws.end));
-            }
             const uint32_t v = vector_width(size, dim, grad, grad_stride, out, out_stride);
-            const uint32_t lanes = lanes_for((dim + v - 1) / v);
+            RunSums a{};
+            a.keys = at(ws.keys[last]);
+            a.rows = at(ws.rows[last]);
+            a.part = reinterpret_cast<float*>(w + ws.part);
+            a.count = ws.count;
+            a.vocab = (uint32_t)vocab;
+            a.dim = dim;
+            a.lanes = lanes_for((dim + v - 1) / v);
+            a.grad_stride = grad_stride;
+            a.out_stride = out_stride;
+            a.scale = scale;
+            const uint32_t groups = kRunThreads / a.lanes, slices = ceil_div(dim, a.lanes * v);
+            // longer chunks mean fewer joins, as long as every SM has a few blocks
+            a.chunk = kMostChunk;
+            while (a.chunk > kAhead && (uint64_t)ceil_div(ws.count, groups * a.chunk) * slices < kFewBlocks) a.chunk /= 2;
+            const dim3 grid(ceil_div(ws.count, groups * a.chunk), slices);
             with_type(type, [&](auto e) {
                 using T = decltype(e);
                 with_width<T>(v, [&](auto wd) {
-                    if constexpr (decltype(wd)::value <= 16 / sizeof(T)) {
+                    constexpr int V = decltype(wd)::value;
+                    if constexpr (V <= 16 / sizeof(T)) {
                         count_launch();
-                        k_run_sums<T, decltype(wd)::value><<<ceil_div(vocab * lanes, 256), 256, 0, s>>>(
-                            static_cast<const T*>(grad), dim, grad_stride, at(ws.rows[last]), at(ws.begin), at(ws.end),
-                            (uint32_t)vocab, scale, static_cast<T*>(out), out_stride, lanes);
+                        k_run_sums<T, V><<<grid, kRunThreads, 0, s>>>(a, static_cast<const T*>(grad),
+                                                                      static_cast<T*>(out));
+                        if (grid.x > 1) {
+                            count_launch();
+                            k_run_joins<T, V><<<grid, kRunThreads, 0, s>>>(a, static_cast<T*>(out));
+                        }
                     }
                 });
             });

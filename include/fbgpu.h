@@ -454,7 +454,7 @@ fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vocab, uint32
  * every one written.  The places are sorted by token (stable), so that each
  * row is summed in f32 in an order that depends on the tokens alone, with no
  * atomics: the same inputs give the same bits.  grad's stride may be 0 (one row
- * for all).  n * per_row and vocab are at most 2^31 - 2.  `workspace` holds
+ * for all).  n * per_row and vocab are at most 2^31 - 2, dim at most 2097120.  `workspace` holds
  * fbgpu_embed_grad_workspace(...) bytes, 256-byte aligned, with any contents. */
 uint64_t fbgpu_embed_grad_workspace(uint64_t n, uint32_t per_row, uint64_t vocab, uint32_t dim);
 fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_t n, uint32_t per_row, uint32_t dim,

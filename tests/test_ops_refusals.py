@@ -56,7 +56,7 @@ def test_embed_refusals(kw, match):
     (dict(tokens=None), "tokens must be"), (dict(out=None), "out must be"), (dict(os=1), "overlap"),
     (dict(out=A), "overlap"), (dict(space=A), "overlap"), (dict(space=E + 128), "256-byte"),
     (dict(size=16), "workspace"), (dict(space=None), "workspace"), (dict(n=1 << 31), "2147483646"),
-    (dict(vocab=1 << 31), "2147483646"),
+    (dict(vocab=1 << 31), "2147483646"), (dict(dim=1 << 22, gs=1 << 22, os=1 << 22), "2097120"),
 ])
 def test_embed_grad_refusals(kw, match):
     refused("fbgpu_embed_grad", *grad(**kw), match=match)
