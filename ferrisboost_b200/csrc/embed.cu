@@ -56,46 +56,64 @@ __global__ void __launch_bounds__(256) k_embed(const T* __restrict__ table, uint
 }
 
 // -------------------------------------------------------------- radix sort
+// The sorted items are (token, row) pairs of 32 bits each.
 constexpr int kSortThreads = 256, kSortItems = 16, kTile = kSortThreads * kSortItems;
 constexpr int kSortWarps = kSortThreads / 32, kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 
-struct SortPass {
-    const uint32_t *keys, *rows;  // null in the first pass, which reads the tokens
-    uint32_t *keys_out, *rows_out;
-    uint32_t* hist;   // [bin][tile]: counts, then offsets within the bin
-    uint32_t* total;  // [bin]
-    uint32_t count, tiles, shift, bins;
+// i / d for i < 2^31: with l = ceil(log2 d), floor(i * (floor(2^(31+l) / d) + 1) / 2^(31+l)), as the excess of the
+// multiplier over 2^(31+l) / d, at most 1, times i stays below 2^31 and so below a unit of the quotient.
+struct Divisor {
+    uint32_t d, mul, shift;
+    explicit Divisor(uint32_t d_ = 1) : d(d_), mul(0), shift(0) {
+        if (d <= 1) return;
+        uint32_t l = 0;
+        while ((1ull << l) < d) l++;
+        mul = (uint32_t)((1ull << (31 + l)) / d + 1);
+        shift = l - 1;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t i) const { return d <= 1 ? i : __umulhi(i, mul) >> shift; }
 };
 
-template <class Tok, bool FIRST>
-__device__ __forceinline__ void load_place(const SortPass& a, const Tokens<Tok>& tokens, uint32_t per_row,
-                                           uint64_t vocab, uint32_t i, uint32_t& key, uint32_t& row) {
-    if (FIRST) {
-        row = i / per_row;
-        key = (uint32_t)tokens.at(row, i - row * per_row, vocab);
-    } else {
-        key = a.keys[i];
-        row = a.rows[i];
+// Where a pass reads its items: the tokens in their order (the first pass), or the items of the pass before.
+template <class Tok> struct Places {
+    Tokens<Tok> tokens;
+    Divisor per_row;
+    uint64_t vocab;
+    __device__ __forceinline__ uint32_t row(uint32_t i) const { return per_row.div(i); }
+    __device__ __forceinline__ uint32_t key(uint32_t i) const {
+        const uint32_t r = row(i);
+        return (uint32_t)tokens.at(r, i - r * per_row.d, vocab);
     }
-}
+};
+
+struct SortPass {
+    const uint2* in;  // not read by the first pass
+    uint2* out;
+    uint32_t* hist;   // [bin][tile]: counts, then offsets within the bin
+    uint32_t* total;  // [bin]
+    uint32_t count, tiles, shift, bits;
+    __device__ __forceinline__ uint32_t digit(uint32_t key) const { return (key >> shift) & ((1u << bits) - 1); }
+};
 
 // Counts each bin of the pass's digit in a tile of 4096 places.
 template <class Tok, bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) k_sort_count(SortPass a, Tokens<Tok> tokens, uint32_t per_row,
-                                                             uint64_t vocab) {
+__global__ void __launch_bounds__(kSortThreads) k_sort_count(SortPass a, Places<Tok> places) {
     __shared__ uint32_t h[kMaxBins];
-    for (uint32_t b = threadIdx.x; b < a.bins; b += kSortThreads) h[b] = 0;
+    const uint32_t bins = 1u << a.bits;
+    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) h[b] = 0;
     __syncthreads();
-    const uint32_t base = blockIdx.x * kTile;
+    const uint32_t base = blockIdx.x * kTile + threadIdx.x;
+    uint32_t key[kSortItems];
+#pragma unroll
     for (int k = 0; k < kSortItems; k++) {
-        const uint32_t i = base + k * kSortThreads + threadIdx.x;
-        if (i >= a.count) break;
-        uint32_t key, row;
-        load_place<Tok, FIRST>(a, tokens, per_row, vocab, i, key, row);
-        atomicAdd(&h[(key >> a.shift) & (a.bins - 1)], 1u);
+        const uint32_t i = base + k * kSortThreads;
+        if (i < a.count) key[k] = FIRST ? places.key(i) : a.in[i].x;
     }
+#pragma unroll
+    for (int k = 0; k < kSortItems; k++)
+        if (base + k * kSortThreads < a.count) atomicAdd(&h[a.digit(key[k])], 1u);
     __syncthreads();
-    for (uint32_t b = threadIdx.x; b < a.bins; b += kSortThreads) a.hist[(uint64_t)b * a.tiles + blockIdx.x] = h[b];
+    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) a.hist[(uint64_t)b * a.tiles + blockIdx.x] = h[b];
 }
 
 // Exclusive sum over the block's threads; `sum` gets the total.
@@ -123,57 +141,86 @@ template <int THREADS> __device__ __forceinline__ uint32_t block_scan(uint32_t v
 // One block per bin: the bin's counts over the tiles become offsets.
 __global__ void __launch_bounds__(kSortThreads) k_sort_scan(SortPass a) {
     __shared__ uint32_t part[kSortWarps];
+    constexpr int kPer = 8;
     uint32_t* h = a.hist + (uint64_t)blockIdx.x * a.tiles;
     uint32_t run = 0;
-    for (uint32_t base = 0; base < a.tiles; base += kSortThreads) {
-        const uint32_t t = base + threadIdx.x;
-        uint32_t sum, v = t < a.tiles ? h[t] : 0;
-        const uint32_t off = block_scan<kSortThreads>(v, part, sum);
-        if (t < a.tiles) h[t] = run + off;
+    for (uint32_t base = 0; base < a.tiles; base += kSortThreads * kPer) {
+        uint32_t v[kPer], mine = 0, sum;
+#pragma unroll
+        for (int k = 0; k < kPer; k++) {
+            const uint32_t t = base + threadIdx.x * kPer + k;
+            v[k] = t < a.tiles ? h[t] : 0;
+            mine += v[k];
+        }
+        uint32_t off = run + block_scan<kSortThreads>(mine, part, sum);
+#pragma unroll
+        for (int k = 0; k < kPer; k++) {
+            const uint32_t t = base + threadIdx.x * kPer + k;
+            if (t < a.tiles) h[t] = off;
+            off += v[k];
+        }
         run += sum;
     }
     if (threadIdx.x == 0) a.total[blockIdx.x] = run;
 }
 
+// The lanes with this lane's digit, among those with `in`: a vote per bit.
+__device__ __forceinline__ uint32_t peers_of(uint32_t digit, uint32_t bits, bool in) {
+    uint32_t peers = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+    for (int b = 0; b < kMaxBits; b++) {
+        if (b >= bits) break;
+        const bool set = digit >> b & 1;
+        const uint32_t vote = __ballot_sync(0xffffffffu, set);
+        peers &= set ? vote : ~vote;
+    }
+    return peers;
+}
+// This lane's number among the warp's items of its digit so far; `seen` counts them per digit.
+__device__ __forceinline__ uint32_t rank_in_warp(uint16_t* seen, uint32_t digit, uint32_t bits, bool in) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t peers = peers_of(digit, bits, in);
+    const uint32_t before = __popc(peers & ((1u << lane) - 1));
+    const uint32_t old = in ? seen[digit] : 0;
+    __syncwarp();
+    if (in && before == 0) seen[digit] = (uint16_t)(old + __popc(peers));
+    __syncwarp();
+    return old + before;
+}
+
 // Moves a tile's places to their bins, in order.  Each warp ranks its 512
-// places 32 at a time by matching digits; the tile is then put in order in
-// shared memory, so that a bin's places are written next to one another.
+// places 32 at a time; the tile is then put in order in shared memory, so that
+// a bin's places are written next to one another.
 template <class Tok, bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) k_sort_scatter(SortPass a, Tokens<Tok> tokens, uint32_t per_row,
-                                                               uint64_t vocab) {
+__global__ void __launch_bounds__(kSortThreads, 4) k_sort_scatter(SortPass a, Places<Tok> places) {
     __shared__ uint16_t seen[kSortWarps][kMaxBins];  // at most kTile
     __shared__ uint32_t first[kMaxBins], dest[kMaxBins];
     __shared__ uint32_t part[kSortWarps];
-    __shared__ uint32_t skey[kTile], srow[kTile];
+    __shared__ uint2 item[kTile];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (uint32_t b = threadIdx.x; b < kSortWarps * kMaxBins; b += kSortThreads) (&seen[0][0])[b] = 0;
-    __syncthreads();
+    const uint32_t bins = 1u << a.bits;
+    for (uint32_t b = threadIdx.x; b < kSortWarps * kMaxBins / 2; b += kSortThreads)
+        reinterpret_cast<uint32_t*>(seen)[b] = 0;
     const uint32_t base = blockIdx.x * kTile, here = min((uint32_t)kTile, a.count - base);
-    uint32_t key[kSortItems], row[kSortItems], rank[kSortItems];
+    const uint32_t mine0 = warp * (kTile / kSortWarps) + lane;
+    uint32_t key[kSortItems], rank[kSortItems];
 #pragma unroll
     for (int k = 0; k < kSortItems; k++) {
-        const uint32_t p = warp * (kTile / kSortWarps) + k * 32 + lane;
-        const bool in = p < here;
-        key[k] = row[k] = 0;
-        if (in) load_place<Tok, FIRST>(a, tokens, per_row, vocab, base + p, key[k], row[k]);
-        const uint32_t d = in ? (key[k] >> a.shift) & (a.bins - 1) : kMaxBins;
-        const uint32_t peers = __match_any_sync(0xffffffffu, d);
-        uint32_t old = 0;
-        const int lead = __ffs(peers) - 1;
-        if (in && lane == lead) {
-            old = seen[warp][d];
-            seen[warp][d] = (uint16_t)(old + __popc(peers));
-        }
-        __syncwarp();
-        rank[k] = __shfl_sync(0xffffffffu, old, lead) + __popc(peers & ((1u << lane) - 1));
+        const uint32_t p = mine0 + k * 32;
+        key[k] = 0;
+        if (p < here) key[k] = FIRST ? places.key(base + p) : a.in[base + p].x;
     }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortItems; k++)
+        rank[k] = rank_in_warp(seen[warp], a.digit(key[k]), a.bits, mine0 + k * 32 < here);
     __syncthreads();
     // where each bin starts in the tile, and where each bin of the tile starts in the output
     uint32_t run = 0, out_run = 0;
-    for (uint32_t b0 = 0; b0 < a.bins; b0 += kSortThreads) {
+    for (uint32_t b0 = 0; b0 < bins; b0 += kSortThreads) {
         const uint32_t b = b0 + threadIdx.x;
         uint32_t mine = 0, all = 0;
-        if (b < a.bins) {
+        if (b < bins) {
             for (int w = 0; w < kSortWarps; w++) {
                 const uint32_t c = seen[w][b];
                 seen[w][b] = (uint16_t)mine;
@@ -184,7 +231,7 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_scatter(SortPass a, Token
         uint32_t sum, out_sum;
         const uint32_t f = block_scan<kSortThreads>(mine, part, sum);
         const uint32_t o = block_scan<kSortThreads>(all, part, out_sum);
-        if (b < a.bins) {
+        if (b < bins) {
             first[b] = run + f;
             dest[b] = out_run + o + a.hist[(uint64_t)b * a.tiles + blockIdx.x];
         }
@@ -194,27 +241,27 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_scatter(SortPass a, Token
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSortItems; k++) {
-        const uint32_t p = warp * (kTile / kSortWarps) + k * 32 + lane;
+        const uint32_t p = mine0 + k * 32;
         if (p < here) {
-            const uint32_t d = (key[k] >> a.shift) & (a.bins - 1);
-            const uint32_t q = first[d] + seen[warp][d] + rank[k];
-            skey[q] = key[k];
-            srow[q] = row[k];
+            const uint32_t d = a.digit(key[k]);
+            item[first[d] + seen[warp][d] + rank[k]] =
+                make_uint2(key[k], FIRST ? places.row(base + p) : a.in[base + p].y);
         }
     }
     __syncthreads();
     for (uint32_t q = threadIdx.x; q < here; q += kSortThreads) {
-        const uint32_t kq = skey[q], d = (kq >> a.shift) & (a.bins - 1);
-        const uint32_t at = dest[d] + (q - first[d]);
-        a.keys_out[at] = kq;
-        a.rows_out[at] = srow[q];
+        const uint2 it = item[q];
+        const uint32_t d = a.digit(it.x);
+        a.out[dest[d] + (q - first[d])] = it;
     }
 }
 
-// A sort of up to CTAS * 8192 places in one launch: the blocks of one cluster
-// hold the places, read one another's digit counts and exchange places through
-// the (L2-resident) buffers.  The remaining blocks of the grid clear the output.
-constexpr int kClusterThreads = 512, kClusterItems = 16, kClusterTile = kClusterThreads * kClusterItems;
+// A sort of up to 8 * 512 * ITEMS places in one launch: the blocks of one
+// cluster hold the places, read one another's digit counts and exchange places
+// through the (L2-resident) buffers.  The remaining blocks of the grid clear the
+// output.
+constexpr int kClusterThreads = 512, kClusterCtas = 8;
+constexpr uint32_t kClusterPlaces = kClusterCtas * kClusterThreads * 16;
 
 struct Clear {
     char* p;          // rows of `bytes` bytes, `stride` bytes apart
@@ -241,57 +288,41 @@ __device__ __forceinline__ void clear_rows(const Clear& z, uint64_t b, uint64_t 
 __global__ void __launch_bounds__(256) k_clear(Clear z) { clear_rows(z, blockIdx.x, gridDim.x); }
 
 struct ClusterSort {
-    uint32_t *keys[2], *rows[2];  // pass p writes set p & 1
+    uint2* items[2];  // pass p writes set p & 1
     uint32_t count, bits, passes;
 };
 
-template <class Tok, int CTAS>
-__global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(ClusterSort a, Tokens<Tok> tokens, uint32_t per_row,
-                                                                  uint64_t vocab, Clear z) {
-    if (blockIdx.x >= CTAS) {
-        clear_rows(z, blockIdx.x - CTAS, gridDim.x - CTAS);
+template <class Tok, int ITEMS>
+__global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(ClusterSort a, Places<Tok> places, Clear z) {
+    if (blockIdx.x >= kClusterCtas) {
+        clear_rows(z, blockIdx.x - kClusterCtas, gridDim.x - kClusterCtas);
         return;
     }
     constexpr int kWarps = kClusterThreads / 32;
     __shared__ uint16_t seen[kWarps][kMaxBins];
     __shared__ uint32_t total[kMaxBins], dest[kMaxBins], part[kWarps];
     const auto cluster = cooperative_groups::this_cluster();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = CTAS == 1 ? 0 : cluster.block_rank();
-    const uint32_t bins = 1u << a.bits, base = cta * kClusterTile + warp * (kClusterTile / kWarps) + lane;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = cluster.block_rank();
+    const uint32_t base = (cta * kWarps + warp) * (32 * ITEMS) + lane, mask = (1u << a.bits) - 1;
+    uint2 *in = nullptr, *out = a.items[0];
     for (uint32_t pass = 0; pass < a.passes; pass++) {
         const uint32_t shift = pass * a.bits;
-        for (uint32_t b = threadIdx.x; b < kWarps * kMaxBins; b += kClusterThreads) (&seen[0][0])[b] = 0;
-        uint32_t key[kClusterItems], row[kClusterItems], rank[kClusterItems];
+        uint32_t rank[ITEMS];
+        uint2 item[ITEMS];
 #pragma unroll
-        for (int k = 0; k < kClusterItems; k++) {
+        for (int k = 0; k < ITEMS; k++) {
             const uint32_t i = base + k * 32;
-            key[k] = row[k] = 0;
-            if (i >= a.count) continue;
-            if (pass == 0) {
-                row[k] = i / per_row;
-                key[k] = (uint32_t)tokens.at(row[k], i - row[k] * per_row, vocab);
-            } else {
-                key[k] = __ldcg(a.keys[(pass - 1) & 1] + i);
-                row[k] = __ldcg(a.rows[(pass - 1) & 1] + i);
-            }
+            item[k] = make_uint2(0, 0);
+            if (i < a.count) item[k] = pass ? __ldcg(in + i) : make_uint2(places.key(i), places.row(i));
         }
+        for (uint32_t b = threadIdx.x; b < kWarps * kMaxBins / 2; b += kClusterThreads)
+            reinterpret_cast<uint32_t*>(seen)[b] = 0;
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kClusterItems; k++) {
-            const bool in = base + k * 32 < a.count;
-            const uint32_t d = in ? (key[k] >> shift) & (bins - 1) : kMaxBins;
-            const uint32_t peers = __match_any_sync(0xffffffffu, d);
-            const int lead = __ffs(peers) - 1;
-            uint32_t old = 0;
-            if (in && lane == lead) {
-                old = seen[warp][d];
-                seen[warp][d] = (uint16_t)(old + __popc(peers));
-            }
-            __syncwarp();
-            rank[k] = __shfl_sync(0xffffffffu, old, lead) + __popc(peers & ((1u << lane) - 1));
-        }
+        for (int k = 0; k < ITEMS; k++)
+            rank[k] = rank_in_warp(seen[warp], (item[k].x >> shift) & mask, a.bits, base + k * 32 < a.count);
         __syncthreads();
-        const uint32_t d = threadIdx.x;  // kMaxBins is the number of threads
+        const uint32_t d = threadIdx.x;  // a thread per bin
         uint32_t mine = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
@@ -300,29 +331,27 @@ __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(ClusterSort a,
             mine += c;
         }
         total[d] = mine;
-        if (CTAS > 1) cluster.sync();
-        uint32_t all = 0, before = 0;
+        cluster.sync();
+        uint32_t all = 0, before = 0, sum;
 #pragma unroll
-        for (int c = 0; c < CTAS; c++) {
-            const uint32_t t = CTAS == 1 ? mine : cluster.map_shared_rank(total, c)[d];
+        for (int c = 0; c < kClusterCtas; c++) {
+            const uint32_t t = cluster.map_shared_rank(total, c)[d];
             all += t;
             if (c < cta) before += t;
         }
-        uint32_t sum;
         dest[d] = before + block_scan<kClusterThreads>(all, part, sum);
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kClusterItems; k++) {
+        for (int k = 0; k < ITEMS; k++) {
             if (base + k * 32 < a.count) {
-                const uint32_t dk = (key[k] >> shift) & (bins - 1);
-                const uint32_t to = dest[dk] + seen[warp][dk] + rank[k];
-                a.keys[pass & 1][to] = key[k];
-                a.rows[pass & 1][to] = row[k];
+                const uint32_t dk = (item[k].x >> shift) & mask;
+                out[dest[dk] + seen[warp][dk] + rank[k]] = item[k];
             }
         }
-        // the places' order is read by every block, and `total` is no longer read
-        if (CTAS > 1) cluster.sync();
-        else __syncthreads();
+        // the items' order is read by every block, and `total` is no longer read
+        cluster.sync();
+        in = out;
+        out = a.items[~pass & 1];
     }
 }
 static_assert(kMaxBins == kClusterThreads, "a thread per bin");
@@ -339,14 +368,14 @@ constexpr int kRunThreads = 256, kAhead = 8;
 constexpr uint32_t kMostChunk = 64, kFewBlocks = 148 * 4, kMostSlices = 65535;
 
 struct RunSums {
-    const uint32_t *keys, *rows;
+    const uint2* items;
     float* part;
     uint32_t count, vocab, dim, lanes, chunk;
     uint64_t grad_stride, out_stride;
     float scale;
 };
 
-__device__ __forceinline__ uint32_t key_at(const RunSums& a, uint64_t i) { return i < a.count ? a.keys[i] : a.vocab; }
+__device__ __forceinline__ uint32_t key_at(const RunSums& a, uint64_t i) { return i < a.count ? a.items[i].x : a.vocab; }
 
 template <class T, int V> __device__ __forceinline__ void write_row(const RunSums& a, T* out, uint32_t key, uint32_t c,
                                                                     const float* acc) {
@@ -372,9 +401,13 @@ __global__ void __launch_bounds__(kRunThreads) k_run_sums(RunSums a, const T* __
         uint32_t key[kAhead], row[kAhead];
         Pack<T, V> g[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            key[k] = key_at(a, begin + p + k);
-            row[k] = key[k] < a.vocab ? a.rows[begin + p + k] : 0;
+        for (int k = 0; k < kAhead; k += 2) {  // the list has room for the last pair
+            const uint64_t i = begin + p + k;
+            const uint4 two = i < a.count ? *reinterpret_cast<const uint4*>(a.items + i) : make_uint4(0, 0, 0, 0);
+            key[k] = i < a.count ? two.x : a.vocab;
+            row[k] = two.y;
+            key[k + 1] = i + 1 < a.count ? two.z : a.vocab;
+            row[k + 1] = two.w;
         }
 #pragma unroll
         for (int k = 0; k < kAhead; k++)
@@ -520,7 +553,7 @@ uint64_t token_extent(uint64_t n, uint64_t per_row, uint64_t row, uint64_t col, 
 
 // Parts of the gradient's workspace, each 256-byte aligned.
 struct GradSpace {
-    uint64_t keys[2], rows[2], hist, total, part, bytes;
+    uint64_t items[2], hist, total, part, bytes;
     uint32_t count, tiles, bits, passes;
     GradSpace(uint64_t n, uint64_t per_row, uint64_t vocab, uint32_t dim) {
         count = (uint32_t)(n * per_row);
@@ -535,7 +568,7 @@ struct GradSpace {
             at += (b + 255) / 256 * 256;
             return p;
         };
-        for (int i = 0; i < 2; i++) keys[i] = take(4ull * count), rows[i] = take(4ull * count);
+        for (int i = 0; i < 2; i++) items[i] = take(8ull * count + 8);  // a last pair is read whole
         hist = take(4ull * (1ull << bits) * tiles);
         total = take(4ull << bits);
         // two rows for each block of k_run_sums; a chunk below the longest is only taken for few blocks
@@ -631,7 +664,7 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
             Clear z{static_cast<char*>(out), vocab, (uint64_t)dim * size, out_stride * size};
             if (out_stride == dim) z = Clear{z.p, 1, vocab * z.bytes, 0};
             const uint64_t cleared = z.rows * ((z.bytes + 15) / 16);
-            if (ws.count == 0 || ws.count > 8 * kClusterTile) {
+            if (ws.count == 0 || ws.count > kClusterPlaces) {
                 count_launch();
                 k_clear<<<(uint32_t)std::min<uint64_t>(148 * 8, (cleared + 255) / 256), 256, 0, s>>>(z);
             }
@@ -639,60 +672,57 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
                 FB_CUDA_CHECK(cudaGetLastError());
                 return;
             }
-            if (ws.count <= 8 * kClusterTile) {
-                ClusterSort a{{at(ws.keys[0]), at(ws.keys[1])}, {at(ws.rows[0]), at(ws.rows[1])}, ws.count, ws.bits,
-                              ws.passes};
-                auto launch = [&](auto ctas) {
-                    constexpr int kCtas = decltype(ctas)::value;
+            const Places<Tok> places{tk, Divisor(per_row), vocab};
+            uint2* items[2] = {reinterpret_cast<uint2*>(w + ws.items[0]), reinterpret_cast<uint2*>(w + ws.items[1])};
+            if (ws.count <= kClusterPlaces) {
+                const ClusterSort a{{items[0], items[1]}, ws.count, ws.bits, ws.passes};
+                auto launch = [&](auto of) {
                     const uint64_t wish = (cleared + 4 * kClusterThreads - 1) / (4 * kClusterThreads);
                     cudaLaunchConfig_t cfg{};
-                    cfg.gridDim = dim3(kCtas + ((uint32_t)std::min<uint64_t>(148 * 3, wish) + kCtas - 1) / kCtas * kCtas);
+                    cfg.gridDim = dim3(kClusterCtas * (1 + ceil_div(std::min<uint64_t>(148 * 3, wish), kClusterCtas)));
                     cfg.blockDim = dim3(kClusterThreads);
                     cfg.stream = s;
                     cudaLaunchAttribute attr{};
                     attr.id = cudaLaunchAttributeClusterDimension;
-                    attr.val.clusterDim.x = kCtas;
+                    attr.val.clusterDim.x = kClusterCtas;
                     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
                     cfg.attrs = &attr;
-                    cfg.numAttrs = kCtas > 1 ? 1 : 0;
+                    cfg.numAttrs = 1;
                     count_launch();
-                    FB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sort_cluster<Tok, kCtas>, a, tk, per_row, vocab, z));
+                    FB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sort_cluster<Tok, decltype(of)::value>, a, places, z));
                 };
-                const uint32_t need = ceil_div(ws.count, kClusterTile);
-                if (need == 1) launch(std::integral_constant<int, 1>{});
-                else if (need == 2) launch(std::integral_constant<int, 2>{});
-                else if (need <= 4) launch(std::integral_constant<int, 4>{});
-                else launch(std::integral_constant<int, 8>{});
+                const uint32_t each = ceil_div(ws.count, kClusterCtas * kClusterThreads);  // places of a thread
+                if (each <= 2) launch(std::integral_constant<int, 2>{});
+                else if (each <= 4) launch(std::integral_constant<int, 4>{});
+                else if (each <= 8) launch(std::integral_constant<int, 8>{});
+                else launch(std::integral_constant<int, 16>{});
             } else {
                 for (uint32_t p = 0; p < ws.passes; p++) {
                     SortPass a{};
-                    a.keys = p ? at(ws.keys[(p - 1) & 1]) : nullptr;
-                    a.rows = p ? at(ws.rows[(p - 1) & 1]) : nullptr;
-                    a.keys_out = at(ws.keys[p & 1]);
-                    a.rows_out = at(ws.rows[p & 1]);
+                    a.in = items[~p & 1];
+                    a.out = items[p & 1];
                     a.hist = at(ws.hist);
                     a.total = at(ws.total);
                     a.count = ws.count;
                     a.tiles = ws.tiles;
                     a.shift = p * ws.bits;
-                    a.bins = 1u << ws.bits;
+                    a.bits = ws.bits;
                     for (int k = 0; k < 3; k++) count_launch();
                     if (p == 0) {
-                        k_sort_count<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
-                        k_sort_scan<<<a.bins, kSortThreads, 0, s>>>(a);
-                        k_sort_scatter<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
+                        k_sort_count<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
+                        k_sort_scan<<<1u << ws.bits, kSortThreads, 0, s>>>(a);
+                        k_sort_scatter<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
                     } else {
-                        k_sort_count<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
-                        k_sort_scan<<<a.bins, kSortThreads, 0, s>>>(a);
-                        k_sort_scatter<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, tk, per_row, vocab);
+                        k_sort_count<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
+                        k_sort_scan<<<1u << ws.bits, kSortThreads, 0, s>>>(a);
+                        k_sort_scatter<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
                     }
                 }
             }
             const int last = (ws.passes - 1) & 1;
             const uint32_t v = vector_width(size, dim, grad, grad_stride, out, out_stride);
             RunSums a{};
-            a.keys = at(ws.keys[last]);
-            a.rows = at(ws.rows[last]);
+            a.items = items[last];
             a.part = reinterpret_cast<float*>(w + ws.part);
             a.count = ws.count;
             a.vocab = (uint32_t)vocab;
