@@ -18,47 +18,21 @@
 namespace fbg {
 namespace {
 
+constexpr uint32_t kMostSlices = 65535;  // of columns: a grid's y extent
+
 template <class Tok> struct Tokens {
     const Tok* p;
     uint64_t row, col;
-    // The token of place (r, j) if it is in [0, vocab), else `vocab`.
+    // The token itself if it is in [0, vocab), else `vocab`; a negative one is above every vocab.
+    __device__ __forceinline__ static uint64_t in(Tok t, uint64_t vocab) {
+        const uint64_t u = (uint64_t)(int64_t)t;
+        return u < vocab ? u : vocab;
+    }
+    // That of place (r, j).
     __device__ __forceinline__ uint64_t at(uint64_t r, uint64_t j, uint64_t vocab) const {
-        const uint64_t t = (uint64_t)(int64_t)p[r * row + j * col];  // a negative token is above every vocab
-        return t < vocab ? t : vocab;
+        return in(p[r * row + j * col], vocab);
     }
 };
-
-// ------------------------------------------------------------------- lookup
-// A group of `lanes` threads (a power of two, at most a warp) makes one output
-// row; lane l holds the elements [V * l, V * l + V) of each slice of V * lanes.
-template <class T, class Tok, int V>
-__global__ void __launch_bounds__(256) k_embed(const T* __restrict__ table, uint64_t vocab, uint32_t dim,
-                                               uint64_t table_stride, Tokens<Tok> tokens, uint64_t n, uint32_t per_row,
-                                               float scale, T* __restrict__ out, uint64_t out_stride, uint32_t lanes) {
-    const uint32_t lane = threadIdx.x & (lanes - 1);
-    const uint64_t groups = (uint64_t)gridDim.x * (blockDim.x / lanes);
-    for (uint64_t r = (uint64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes; r < n; r += groups) {
-        for (uint32_t c = lane * V; c < dim; c += lanes * V) {
-            float acc[V] = {};
-            for (uint32_t j = 0; j < per_row; j++) {
-                const uint64_t t = tokens.at(r, j, vocab);
-                if (t >= vocab) continue;
-                const Pack<T, V> e = *reinterpret_cast<const Pack<T, V>*>(table + t * table_stride + c);
-#pragma unroll
-                for (int i = 0; i < V; i++) acc[i] += to_f32(e.v[i]);
-            }
-            Pack<T, V> o;
-#pragma unroll
-            for (int i = 0; i < V; i++) o.v[i] = from_f32<T>(acc[i] * scale);
-            *reinterpret_cast<Pack<T, V>*>(out + r * out_stride + c) = o;
-        }
-    }
-}
-
-// -------------------------------------------------------------- radix sort
-// The sorted items are (token, row) pairs of 32 bits each.
-constexpr int kSortThreads = 256, kSortItems = 16, kTile = kSortThreads * kSortItems;
-constexpr int kSortWarps = kSortThreads / 32, kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 
 // i / d for i < 2^31: with l = ceil(log2 d), floor(i * (floor(2^(31+l) / d) + 1) / 2^(31+l)), as the excess of the
 // multiplier over 2^(31+l) / d, at most 1, times i stays below 2^31 and so below a unit of the quotient.
@@ -74,13 +48,159 @@ struct Divisor {
     __device__ __forceinline__ uint32_t div(uint32_t i) const { return d <= 1 ? i : __umulhi(i, mul) >> shift; }
 };
 
+// A vector of f32 sums.  Pairs are added by one instruction (add.rn.f32x2), each
+// half rounded as an addition of its own.
+template <int V> struct Sums {
+    float v[V];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = 0.0f;
+    }
+    __device__ __forceinline__ void add(int i, float a, float b) {
+        asm("{.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\t"
+            "mov.b64 {%0, %1}, x;}"
+            : "+f"(v[i]), "+f"(v[i + 1])
+            : "f"(a), "f"(b));
+    }
+    __device__ __forceinline__ void add(const float* o) {
+#pragma unroll
+        for (int i = 0; i + 1 < V; i += 2) add(i, o[i], o[i + 1]);
+        if (V & 1) v[V - 1] += o[V - 1];
+    }
+    template <class T> __device__ __forceinline__ void add(const Pack<T, V>& p) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) o[i] = to_f32(p.v[i]);
+        add(o);
+    }
+    template <class T> __device__ __forceinline__ Pack<T, V> scaled(float scale) const {
+        Pack<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++) o.v[i] = from_f32<T>(v[i] * scale);
+        return o;
+    }
+};
+
+// ------------------------------------------------------------------- lookup
+// One token a row: a copy with a scale, memory bound.  The output's vectors are
+// taken in order, four a thread, so that four loads are in flight and what a
+// warp writes is contiguous.
+constexpr int kLookupThreads = 256, kLookupItems = 4;
+
+struct LookupArgs {
+    uint64_t vocab, table_stride, n, out_stride;
+    uint32_t dim;
+    Divisor vectors;  // of a row
+    float scale;
+};
+
+template <class T, class Tok, int V>
+__global__ void __launch_bounds__(kLookupThreads) k_lookup(LookupArgs a, const T* __restrict__ table,
+                                                           Tokens<Tok> tokens, T* __restrict__ out) {
+    constexpr uint32_t kSpan = kLookupThreads * kLookupItems;
+    const uint64_t spans = (a.n * a.vectors.d + kSpan - 1) / kSpan;
+    for (uint64_t s = blockIdx.x; s < spans; s += gridDim.x) {
+        const uint64_t r0 = s * kSpan / a.vectors.d;
+        const uint32_t off = (uint32_t)(s * kSpan - r0 * a.vectors.d) + threadIdx.x;
+        uint64_t at[kLookupItems], token[kLookupItems];
+        Pack<T, V> e[kLookupItems];
+#pragma unroll
+        for (int k = 0; k < kLookupItems; k++) {
+            const uint32_t i = off + k * kLookupThreads, r = a.vectors.div(i), c = (i - r * a.vectors.d) * V;
+            const bool in = r0 + r < a.n;
+            token[k] = in ? tokens.at(r0 + r, 0, a.vocab) : a.vocab;
+            at[k] = in ? (r0 + r) * a.out_stride + c : ~0ull;
+            if (token[k] < a.vocab)
+                e[k] = *reinterpret_cast<const Pack<T, V>*>(table + token[k] * a.table_stride + c);
+        }
+#pragma unroll
+        for (int k = 0; k < kLookupItems; k++) {
+            if (at[k] == ~0ull) continue;
+            Sums<V> sum;
+            sum.clear();
+            if (token[k] < a.vocab) sum.add(e[k]);
+            *reinterpret_cast<Pack<T, V>*>(out + at[k]) = sum.template scaled<T>(a.scale);
+        }
+    }
+}
+
+// Several tokens a row: a group of `lanes` threads (a power of two, at most a
+// warp) sums a slice of V * lanes columns over the tokens of a row, or of one of
+// its `parts` parts, eight loads in flight; a row's parts are neighbours in
+// their block and are joined in order.
+constexpr int kBagThreads = 256, kBagAhead = 8;
+
+struct BagArgs {
+    uint64_t vocab, table_stride, n, out_stride;
+    uint32_t dim, per_row, part_len;
+    uint32_t lanes_log, parts_log;
+    float scale;
+};
+
+template <class T, class Tok, int V>
+__global__ void __launch_bounds__(kBagThreads) k_embed(BagArgs a, const T* __restrict__ table, Tokens<Tok> tokens,
+                                                       T* __restrict__ out) {
+    __shared__ float joined[kBagThreads * V];
+    const uint32_t lane = threadIdx.x & ((1u << a.lanes_log) - 1);
+    const uint32_t part = threadIdx.x >> a.lanes_log & ((1u << a.parts_log) - 1);
+    const uint32_t rows = kBagThreads >> (a.lanes_log + a.parts_log);  // of a block
+    const uint32_t c = (((uint32_t)blockIdx.y << a.lanes_log) + lane) * V;
+    const uint32_t begin = min(part * a.part_len, a.per_row), end = min(begin + a.part_len, a.per_row);
+    for (uint64_t r0 = (uint64_t)blockIdx.x * rows; r0 < a.n; r0 += (uint64_t)gridDim.x * rows) {
+        const uint64_t r = r0 + (threadIdx.x >> (a.lanes_log + a.parts_log));
+        Sums<V> sum;
+        sum.clear();
+        if (r < a.n && c < a.dim) {
+            const Tok* tok = tokens.p + r * tokens.row;
+            for (uint32_t j = begin; j < end; j += kBagAhead) {
+                uint64_t t[kBagAhead];
+                Pack<T, V> e[kBagAhead];
+#pragma unroll
+                for (int k = 0; k < kBagAhead; k++)
+                    t[k] = j + k < end ? tokens.in(tok[(j + k) * tokens.col], a.vocab) : a.vocab;
+#pragma unroll
+                for (int k = 0; k < kBagAhead; k++) {
+                    if (t[k] < a.vocab)
+                        e[k] = *reinterpret_cast<const Pack<T, V>*>(table + t[k] * a.table_stride + c);
+                }
+#pragma unroll
+                for (int k = 0; k < kBagAhead; k++)
+                    if (t[k] < a.vocab) sum.add(e[k]);
+            }
+        }
+        if (a.parts_log) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < V; i++) joined[i * kBagThreads + threadIdx.x] = sum.v[i];
+            __syncthreads();
+            if (part == 0) {
+                for (uint32_t p = 1; p < 1u << a.parts_log; p++) {
+                    float o[V];
+#pragma unroll
+                    for (int i = 0; i < V; i++) o[i] = joined[i * kBagThreads + threadIdx.x + (p << a.lanes_log)];
+                    sum.add(o);
+                }
+            }
+        }
+        if (part == 0 && r < a.n && c < a.dim)
+            *reinterpret_cast<Pack<T, V>*>(out + r * a.out_stride + c) = sum.template scaled<T>(a.scale);
+    }
+}
+
+// -------------------------------------------------------------- radix sort
+// The sorted items are (token, row) pairs of 32 bits each.
+constexpr int kSortThreads = 256, kSortItems = 16, kTile = kSortThreads * kSortItems;
+constexpr int kSortWarps = kSortThreads / 32, kMaxBits = 9, kMaxBins = 1 << kMaxBits;
+
 // Where a pass reads its items: the tokens in their order (the first pass), or the items of the pass before.
 template <class Tok> struct Places {
     Tokens<Tok> tokens;
     Divisor per_row;
     uint64_t vocab;
+    bool flat;  // place i is at tokens + i
     __device__ __forceinline__ uint32_t row(uint32_t i) const { return per_row.div(i); }
     __device__ __forceinline__ uint32_t key(uint32_t i) const {
+        if (flat) return (uint32_t)tokens.in(tokens.p[i], vocab);
         const uint32_t r = row(i);
         return (uint32_t)tokens.at(r, i - r * per_row.d, vocab);
     }
@@ -365,7 +485,7 @@ static_assert(kMaxBins == kClusterThreads, "a thread per bin");
 // goes on through.  What leaves the block is kept in `part`: [block][0] the sum
 // of the run that came in, [block][1] of the one that goes out.
 constexpr int kRunThreads = 256, kAhead = 8;
-constexpr uint32_t kMostChunk = 64, kFewBlocks = 148 * 4, kMostSlices = 65535;
+constexpr uint32_t kMostChunk = 64, kFewBlocks = 148 * 4;
 
 struct RunSums {
     const uint2* items;
@@ -378,11 +498,8 @@ struct RunSums {
 __device__ __forceinline__ uint32_t key_at(const RunSums& a, uint64_t i) { return i < a.count ? a.items[i].x : a.vocab; }
 
 template <class T, int V> __device__ __forceinline__ void write_row(const RunSums& a, T* out, uint32_t key, uint32_t c,
-                                                                    const float* acc) {
-    Pack<T, V> o;
-#pragma unroll
-    for (int k = 0; k < V; k++) o.v[k] = from_f32<T>(acc[k] * a.scale);
-    *reinterpret_cast<Pack<T, V>*>(out + key * a.out_stride + c) = o;
+                                                                    const Sums<V>& sum) {
+    *reinterpret_cast<Pack<T, V>*>(out + key * a.out_stride + c) = sum.template scaled<T>(a.scale);
 }
 
 template <class T, int V>
@@ -396,7 +513,8 @@ __global__ void __launch_bounds__(kRunThreads) k_run_sums(RunSums a, const T* __
     uint32_t cur = key_at(a, begin);
     const bool from_before = begin > 0 && cur < a.vocab && key_at(a, begin - 1) == cur;
     bool head = from_before;  // the current run is the one that came in
-    float acc[V] = {};
+    Sums<V> acc;
+    acc.clear();
     for (uint32_t p = 0; p < a.chunk; p += kAhead) {
         uint32_t key[kAhead], row[kAhead];
         Pack<T, V> g[kAhead];
@@ -418,25 +536,21 @@ __global__ void __launch_bounds__(kRunThreads) k_run_sums(RunSums a, const T* __
             if (key[k] != cur) {
                 if (head) {
 #pragma unroll
-                    for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc[i];
+                    for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc.v[i];
                 } else if (column) {
                     write_row<T, V>(a, out, cur, c, acc);
                 }
                 head = false;
                 cur = key[k];
-#pragma unroll
-                for (int i = 0; i < V; i++) acc[i] = 0.0f;
+                acc.clear();
             }
-            if (column && key[k] < a.vocab) {
-#pragma unroll
-                for (int i = 0; i < V; i++) acc[i] += to_f32(g[k].v[i]);
-            }
+            if (column && key[k] < a.vocab) acc.add(g[k]);
         }
     }
     const bool to_after = cur < a.vocab && key_at(a, begin + a.chunk) == cur;
     if (head) {
 #pragma unroll
-        for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc[i];
+        for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc.v[i];
     } else if (!to_after && cur < a.vocab && column) {
         write_row<T, V>(a, out, cur, c, acc);
     }
@@ -447,29 +561,28 @@ __global__ void __launch_bounds__(kRunThreads) k_run_sums(RunSums a, const T* __
         uint32_t h = group + 1;
         bool open = true;
         for (; h < groups && open; h++) {
-#pragma unroll
-            for (int i = 0; i < V; i++) acc[i] += heads[(h * a.lanes + lane) * V + i];
+            acc.add(heads + (h * a.lanes + lane) * V);
             open = goes_on[h];
         }
         if (column) {
             if (open) {
 #pragma unroll
-                for (int i = 0; i < V; i++) a.part[block + a.dim + c + i] = acc[i];
+                for (int i = 0; i < V; i++) a.part[block + a.dim + c + i] = acc.v[i];
             } else {
                 write_row<T, V>(a, out, cur, c, acc);
             }
         }
     }
     if (group == 0 && from_before && column) {  // the run that came into the block
-        float sum[V] = {};
+        Sums<V> sum;
+        sum.clear();
         bool open = true;
         for (uint32_t h = 0; h < groups && open; h++) {
-#pragma unroll
-            for (int i = 0; i < V; i++) sum[i] += heads[(h * a.lanes + lane) * V + i];
+            sum.add(heads + (h * a.lanes + lane) * V);
             open = goes_on[h];
         }
 #pragma unroll
-        for (int i = 0; i < V; i++) a.part[block + c + i] = sum[i];
+        for (int i = 0; i < V; i++) a.part[block + c + i] = sum.v[i];
     }
 }
 
@@ -492,27 +605,22 @@ __global__ void __launch_bounds__(kRunThreads) k_run_joins(RunSums a, T* __restr
     }
     const uint32_t c = (blockIdx.y * a.lanes + lane) * V;
     const bool column = c < a.dim;
-    float acc[V] = {};
+    Sums<V> acc;
+    acc.clear();
     if (column) {
         const float* part = a.part + (uint64_t)blockIdx.x * 2 * a.dim + c;
         if (group == 0) {
 #pragma unroll
-            for (int i = 0; i < V; i++) acc[i] = part[a.dim + i];
+            for (int i = 0; i < V; i++) acc.v[i] = part[a.dim + i];
         }
 #pragma unroll 4
-        for (uint32_t b = 1 + group; b <= more; b += groups) {
-#pragma unroll
-            for (int i = 0; i < V; i++) acc[i] += part[(uint64_t)b * 2 * a.dim + i];
-        }
+        for (uint32_t b = 1 + group; b <= more; b += groups) acc.add(part + (uint64_t)b * 2 * a.dim);
     }
 #pragma unroll
-    for (int i = 0; i < V; i++) sums[threadIdx.x * V + i] = acc[i];
+    for (int i = 0; i < V; i++) sums[threadIdx.x * V + i] = acc.v[i];
     __syncthreads();
     if (group == 0 && column) {
-        for (uint32_t h = 1; h < groups && h <= more; h++) {
-#pragma unroll
-            for (int i = 0; i < V; i++) acc[i] += sums[(h * a.lanes + lane) * V + i];
-        }
+        for (uint32_t h = 1; h < groups && h <= more; h++) acc.add(sums + (h * a.lanes + lane) * V);
         write_row<T, V>(a, out, key, c, acc);
     }
 }
@@ -527,12 +635,11 @@ uint32_t vector_width(uint32_t size, uint64_t dim, const void* a, uint64_t a_str
     return v;
 }
 template <class T, class F> void with_width(uint32_t v, F&& f) {
-    switch (v) {
-        case 1: f(std::integral_constant<int, 1>{}); break;
-        case 2: f(std::integral_constant<int, 2>{}); break;
-        case 4: f(std::integral_constant<int, 4>{}); break;
-        default: f(std::integral_constant<int, 16 / sizeof(T)>{}); break;
-    }
+    constexpr int kMost = 16 / sizeof(T);
+    if (v == 1) f(std::integral_constant<int, 1>{});
+    else if (v == 2) f(std::integral_constant<int, 2>{});
+    else if (v == 4) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, kMost>{});
 }
 uint32_t lanes_for(uint64_t chunks) {
     uint32_t lanes = 1;
@@ -605,21 +712,42 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
                 throw InputError("out must not overlap the table or the tokens");
             cudaStream_t s = check_stream(stream);
             if (!n || !dim) return;
-            const uint32_t v = vector_width(size, dim, table, table_stride, out, out_stride);
-            const uint32_t lanes = lanes_for((dim + v - 1) / v);
-            const uint32_t blocks = (uint32_t)std::min<uint64_t>(1u << 20, (n * lanes + 255) / 256);
-            with_type(type, [&](auto e) {
-                using T = decltype(e);
-                with_width<T>(v, [&](auto w) {
-                    if constexpr (decltype(w)::value <= 16 / sizeof(T)) {
-                        count_launch();
-                        k_embed<T, Tok, decltype(w)::value><<<blocks, 256, 0, s>>>(
-                            static_cast<const T*>(table), vocab, dim, table_stride,
-                            Tokens<Tok>{static_cast<const Tok*>(tokens), token_row, token_col}, n, per_row, scale,
-                            static_cast<T*>(out), out_stride, lanes);
-                    }
+            const uint32_t v = vector_width(size, dim, table, table_stride, out, out_stride), vectors = (dim + v - 1) / v;
+            const Tokens<Tok> tk{static_cast<const Tok*>(tokens), token_row, token_col};
+            if (per_row == 1 && vectors < 1u << 30) {
+                const LookupArgs a{vocab, table_stride, n, out_stride, dim, Divisor(vectors), scale};
+                constexpr uint64_t kSpan = kLookupThreads * kLookupItems;
+                const uint64_t spans = n > (1ull << 40) / vectors ? 1u << 20 : (n * vectors + kSpan - 1) / kSpan;
+                const uint32_t blocks = (uint32_t)std::min<uint64_t>(1u << 20, spans);
+                with_type(type, [&](auto e) {
+                    using T = decltype(e);
+                    with_width<T>(v, [&](auto w) {
+                        k_lookup<T, Tok, decltype(w)::value><<<blocks, kLookupThreads, 0, s>>>(
+                            a, static_cast<const T*>(table), tk, static_cast<T*>(out));
+                    });
                 });
-            });
+            } else {
+                BagArgs a{vocab, table_stride, n, out_stride, dim, per_row, per_row, 0, 0, scale};
+                while (1u << a.lanes_log < lanes_for(vectors)) a.lanes_log++;
+                const uint32_t slices = ceil_div(vectors, 1u << a.lanes_log);
+                if (slices > kMostSlices) throw InputError("fbgpu_embed takes rows of at most 2097120 elements");
+                // parts of a row, until every SM has about a thousand threads; a part has at least eight tokens
+                while (a.lanes_log + a.parts_log < 8 && a.part_len > kBagAhead &&
+                       n < (148ull * 1024 >> (a.lanes_log + a.parts_log)) / slices) {
+                    a.parts_log++;
+                    a.part_len = ceil_div(per_row, 1u << a.parts_log);
+                }
+                const uint32_t rows = kBagThreads >> (a.lanes_log + a.parts_log);
+                const dim3 grid((uint32_t)std::min<uint64_t>(1u << 20, (n + rows - 1) / rows), slices);
+                with_type(type, [&](auto e) {
+                    using T = decltype(e);
+                    with_width<T>(v, [&](auto w) {
+                        k_embed<T, Tok, decltype(w)::value><<<grid, kBagThreads, 0, s>>>(
+                            a, static_cast<const T*>(table), tk, static_cast<T*>(out));
+                    });
+                });
+            }
+            count_launch();
             FB_CUDA_CHECK(cudaGetLastError());
         });
     });
@@ -672,7 +800,8 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
                 FB_CUDA_CHECK(cudaGetLastError());
                 return;
             }
-            const Places<Tok> places{tk, Divisor(per_row), vocab};
+            const Places<Tok> places{tk, Divisor(per_row), vocab,
+                                     (per_row == 1 || token_col == 1) && (n == 1 || token_row == per_row)};
             uint2* items[2] = {reinterpret_cast<uint2*>(w + ws.items[0]), reinterpret_cast<uint2*>(w + ws.items[1])};
             if (ws.count <= kClusterPlaces) {
                 const ClusterSort a{{items[0], items[1]}, ws.count, ws.bits, ws.passes};
@@ -740,14 +869,11 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
                 using T = decltype(e);
                 with_width<T>(v, [&](auto wd) {
                     constexpr int V = decltype(wd)::value;
-                    if constexpr (V <= 16 / sizeof(T)) {
+                    count_launch();
+                    k_run_sums<T, V><<<grid, kRunThreads, 0, s>>>(a, static_cast<const T*>(grad), static_cast<T*>(out));
+                    if (grid.x > 1) {
                         count_launch();
-                        k_run_sums<T, V><<<grid, kRunThreads, 0, s>>>(a, static_cast<const T*>(grad),
-                                                                      static_cast<T*>(out));
-                        if (grid.x > 1) {
-                            count_launch();
-                            k_run_joins<T, V><<<grid, kRunThreads, 0, s>>>(a, static_cast<T*>(out));
-                        }
+                        k_run_joins<T, V><<<grid, kRunThreads, 0, s>>>(a, static_cast<T*>(out));
                     }
                 });
             });
