@@ -11,6 +11,8 @@
 // written at once; what continues into another part is joined from the parts'
 // sums in a second pass.  No atomics: the order of every sum follows from the
 // tokens and the sizes.
+#include <type_traits>
+
 #include <cooperative_groups.h>
 
 #include "ops.h"
@@ -20,18 +22,20 @@ namespace {
 
 constexpr uint32_t kMostSlices = 65535;  // of columns: a grid's y extent
 
+// What a missing token's lookup reads.
+__device__ __align__(16) const uint4 g_zero{0, 0, 0, 0};
+
 template <class Tok> struct Tokens {
+    // Tokens as unsigned numbers of their own width: a negative one is above every `vocab`, which is at most
+    // 2^31 (2^63), as no token of the type is larger.
+    using U = std::make_unsigned_t<Tok>;
     const Tok* p;
     uint64_t row, col;
-    // The token itself if it is in [0, vocab), else `vocab`; a negative one is above every vocab.
-    __device__ __forceinline__ static uint64_t in(Tok t, uint64_t vocab) {
-        const uint64_t u = (uint64_t)(int64_t)t;
-        return u < vocab ? u : vocab;
-    }
-    // That of place (r, j).
-    __device__ __forceinline__ uint64_t at(uint64_t r, uint64_t j, uint64_t vocab) const {
-        return in(p[r * row + j * col], vocab);
-    }
+    U vocab;
+    Tokens(const void* p_, uint64_t row_, uint64_t col_, uint64_t vocab_)
+        : p(static_cast<const Tok*>(p_)), row(row_), col(col_),
+          vocab((U)std::min<uint64_t>(vocab_, 1ull << (8 * sizeof(Tok) - 1))) {}
+    __device__ __forceinline__ U at(uint64_t r, uint64_t j) const { return (U)p[r * row + j * col]; }
 };
 
 // i / d for i < 2^31: with l = ceil(log2 d), floor(i * (floor(2^(31+l) / d) + 1) / 2^(31+l)), as the excess of the
@@ -82,64 +86,69 @@ template <int V> struct Sums {
 };
 
 // ------------------------------------------------------------------- lookup
-// One token a row: a copy with a scale, memory bound.  The output's vectors are
-// taken in order, four a thread, so that four loads are in flight and what a
-// warp writes is contiguous.
-constexpr int kLookupThreads = 256, kLookupItems = 4;
+// One token a row: a copy with a scale, memory bound.  A group of `lanes`
+// threads takes four rows at a time, so that four loads are in flight and a
+// token is read once a row.
+constexpr int kLookupThreads = 256, kLookupRows = 4;
 
 struct LookupArgs {
-    uint64_t vocab, table_stride, n, out_stride;
-    uint32_t dim;
-    Divisor vectors;  // of a row
+    uint64_t table_stride, n, out_stride;
+    uint32_t dim, lanes_log;
     float scale;
 };
 
 template <class T, class Tok, int V>
 __global__ void __launch_bounds__(kLookupThreads) k_lookup(LookupArgs a, const T* __restrict__ table,
                                                            Tokens<Tok> tokens, T* __restrict__ out) {
-    constexpr uint32_t kSpan = kLookupThreads * kLookupItems;
-    const uint64_t spans = (a.n * a.vectors.d + kSpan - 1) / kSpan;
-    for (uint64_t s = blockIdx.x; s < spans; s += gridDim.x) {
-        const uint64_t r0 = s * kSpan / a.vectors.d;
-        const uint32_t off = (uint32_t)(s * kSpan - r0 * a.vectors.d) + threadIdx.x;
-        uint64_t at[kLookupItems], token[kLookupItems];
-        Pack<T, V> e[kLookupItems];
+    using P = Pack<T, V>;
+    const uint64_t groups = (uint64_t)gridDim.x * (kLookupThreads >> a.lanes_log);
+    const uint32_t lane = threadIdx.x & ((1u << a.lanes_log) - 1);
+    for (uint64_t r = ((uint64_t)blockIdx.x * kLookupThreads + threadIdx.x) >> a.lanes_log; r < a.n;
+         r += kLookupRows * groups) {
+        const T* from[kLookupRows];
+        T* to[kLookupRows];
 #pragma unroll
-        for (int k = 0; k < kLookupItems; k++) {
-            const uint32_t i = off + k * kLookupThreads, r = a.vectors.div(i), c = (i - r * a.vectors.d) * V;
-            const bool in = r0 + r < a.n;
-            token[k] = in ? tokens.at(r0 + r, 0, a.vocab) : a.vocab;
-            at[k] = in ? (r0 + r) * a.out_stride + c : ~0ull;
-            if (token[k] < a.vocab)
-                e[k] = *reinterpret_cast<const Pack<T, V>*>(table + token[k] * a.table_stride + c);
+        for (int k = 0; k < kLookupRows; k++) {
+            from[k] = nullptr;
+            to[k] = r + k * groups < a.n ? out + (r + k * groups) * a.out_stride : nullptr;
+            if (!to[k]) continue;
+            const auto t = tokens.at(r + k * groups, 0);
+            if (t < tokens.vocab) from[k] = table + t * a.table_stride;
         }
+        for (uint32_t c = lane * V; c < a.dim; c += V << a.lanes_log) {
+            P e[kLookupRows];
 #pragma unroll
-        for (int k = 0; k < kLookupItems; k++) {
-            if (at[k] == ~0ull) continue;
-            Sums<V> sum;
-            sum.clear();
-            if (token[k] < a.vocab) sum.add(e[k]);
-            *reinterpret_cast<Pack<T, V>*>(out + at[k]) = sum.template scaled<T>(a.scale);
+            for (int k = 0; k < kLookupRows; k++)
+                e[k] = *(from[k] ? reinterpret_cast<const P*>(from[k] + c) : reinterpret_cast<const P*>(&g_zero));
+#pragma unroll
+            for (int k = 0; k < kLookupRows; k++) {
+                Sums<V> sum;
+                sum.clear();
+                sum.add(e[k]);
+                if (to[k]) *reinterpret_cast<P*>(to[k] + c) = sum.template scaled<T>(a.scale);
+            }
         }
     }
 }
 
 // Several tokens a row: a group of `lanes` threads (a power of two, at most a
 // warp) sums a slice of V * lanes columns over the tokens of a row, or of one of
-// its `parts` parts, eight loads in flight; a row's parts are neighbours in
-// their block and are joined in order.
+// its `parts` parts, eight loads in flight and the next eight tokens behind
+// them; a row's parts are neighbours in their block and are joined in order.
 constexpr int kBagThreads = 256, kBagAhead = 8;
 
 struct BagArgs {
-    uint64_t vocab, table_stride, n, out_stride;
+    uint64_t table_stride, n, out_stride;
     uint32_t dim, per_row, part_len;
     uint32_t lanes_log, parts_log;
     float scale;
 };
 
 template <class T, class Tok, int V>
-__global__ void __launch_bounds__(kBagThreads) k_embed(BagArgs a, const T* __restrict__ table, Tokens<Tok> tokens,
-                                                       T* __restrict__ out) {
+__global__ void __launch_bounds__(kBagThreads, 4) k_embed(BagArgs a, const T* __restrict__ table, Tokens<Tok> tokens,
+                                                          T* __restrict__ out) {
+    using P = Pack<T, V>;
+    using U = typename Tokens<Tok>::U;
     __shared__ float joined[kBagThreads * V];
     const uint32_t lane = threadIdx.x & ((1u << a.lanes_log) - 1);
     const uint32_t part = threadIdx.x >> a.lanes_log & ((1u << a.parts_log) - 1);
@@ -152,20 +161,24 @@ __global__ void __launch_bounds__(kBagThreads) k_embed(BagArgs a, const T* __res
         sum.clear();
         if (r < a.n && c < a.dim) {
             const Tok* tok = tokens.p + r * tokens.row;
+            const T* column = table + c;
+            U t[kBagAhead];
+#pragma unroll
+            for (int k = 0; k < kBagAhead; k++)
+                t[k] = begin + k < end ? (U)tok[(begin + k) * tokens.col] : tokens.vocab;
             for (uint32_t j = begin; j < end; j += kBagAhead) {
-                uint64_t t[kBagAhead];
-                Pack<T, V> e[kBagAhead];
+                P e[kBagAhead];
 #pragma unroll
                 for (int k = 0; k < kBagAhead; k++)
-                    t[k] = j + k < end ? tokens.in(tok[(j + k) * tokens.col], a.vocab) : a.vocab;
+                    e[k] = *(t[k] < tokens.vocab ? reinterpret_cast<const P*>(column + t[k] * a.table_stride)
+                                                 : reinterpret_cast<const P*>(&g_zero));
 #pragma unroll
                 for (int k = 0; k < kBagAhead; k++) {
-                    if (t[k] < a.vocab)
-                        e[k] = *reinterpret_cast<const Pack<T, V>*>(table + t[k] * a.table_stride + c);
+                    const uint32_t next = j + kBagAhead + k;
+                    t[k] = next < end ? (U)tok[next * tokens.col] : tokens.vocab;
                 }
 #pragma unroll
-                for (int k = 0; k < kBagAhead; k++)
-                    if (t[k] < a.vocab) sum.add(e[k]);
+                for (int k = 0; k < kBagAhead; k++) sum.add(e[k]);
             }
         }
         if (a.parts_log) {
@@ -183,7 +196,7 @@ __global__ void __launch_bounds__(kBagThreads) k_embed(BagArgs a, const T* __res
             }
         }
         if (part == 0 && r < a.n && c < a.dim)
-            *reinterpret_cast<Pack<T, V>*>(out + r * a.out_stride + c) = sum.template scaled<T>(a.scale);
+            *reinterpret_cast<P*>(out + r * a.out_stride + c) = sum.template scaled<T>(a.scale);
     }
 }
 
@@ -192,17 +205,22 @@ __global__ void __launch_bounds__(kBagThreads) k_embed(BagArgs a, const T* __res
 constexpr int kSortThreads = 256, kSortItems = 16, kTile = kSortThreads * kSortItems;
 constexpr int kSortWarps = kSortThreads / 32, kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 
-// Where a pass reads its items: the tokens in their order (the first pass), or the items of the pass before.
+// Where a pass reads its items: from the pass before, or, the first, from the
+// tokens, place i being at tokens + i where they are flat.
+enum Source { kItems, kFlat, kStrided };
 template <class Tok> struct Places {
     Tokens<Tok> tokens;
     Divisor per_row;
-    uint64_t vocab;
-    bool flat;  // place i is at tokens + i
     __device__ __forceinline__ uint32_t row(uint32_t i) const { return per_row.div(i); }
-    __device__ __forceinline__ uint32_t key(uint32_t i) const {
-        if (flat) return (uint32_t)tokens.in(tokens.p[i], vocab);
-        const uint32_t r = row(i);
-        return (uint32_t)tokens.at(r, i - r * per_row.d, vocab);
+    template <Source S> __device__ __forceinline__ uint32_t key(uint32_t i) const {
+        typename Tokens<Tok>::U t;
+        if (S == kFlat) {
+            t = tokens.p[i];
+        } else {
+            const uint32_t r = row(i);
+            t = tokens.at(r, i - r * per_row.d);
+        }
+        return (uint32_t)min(t, tokens.vocab);
     }
 };
 
@@ -216,7 +234,7 @@ struct SortPass {
 };
 
 // Counts each bin of the pass's digit in a tile of 4096 places.
-template <class Tok, bool FIRST>
+template <class Tok, Source S>
 __global__ void __launch_bounds__(kSortThreads) k_sort_count(SortPass a, Places<Tok> places) {
     __shared__ uint32_t h[kMaxBins];
     const uint32_t bins = 1u << a.bits;
@@ -227,7 +245,9 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_count(SortPass a, Places<
 #pragma unroll
     for (int k = 0; k < kSortItems; k++) {
         const uint32_t i = base + k * kSortThreads;
-        if (i < a.count) key[k] = FIRST ? places.key(i) : a.in[i].x;
+        const uint32_t q = min(i, a.count - 1);
+        if constexpr (S == kItems) key[k] = a.in[q].x;
+        else key[k] = places.template key<S>(q);
     }
 #pragma unroll
     for (int k = 0; k < kSortItems; k++)
@@ -311,7 +331,7 @@ __device__ __forceinline__ uint32_t rank_in_warp(uint16_t* seen, uint32_t digit,
 // Moves a tile's places to their bins, in order.  Each warp ranks its 512
 // places 32 at a time; the tile is then put in order in shared memory, so that
 // a bin's places are written next to one another.
-template <class Tok, bool FIRST>
+template <class Tok, Source S>
 __global__ void __launch_bounds__(kSortThreads, 4) k_sort_scatter(SortPass a, Places<Tok> places) {
     __shared__ uint16_t seen[kSortWarps][kMaxBins];  // at most kTile
     __shared__ uint32_t first[kMaxBins], dest[kMaxBins];
@@ -327,8 +347,9 @@ __global__ void __launch_bounds__(kSortThreads, 4) k_sort_scatter(SortPass a, Pl
 #pragma unroll
     for (int k = 0; k < kSortItems; k++) {
         const uint32_t p = mine0 + k * 32;
-        key[k] = 0;
-        if (p < here) key[k] = FIRST ? places.key(base + p) : a.in[base + p].x;
+        const uint32_t q = base + min(p, here - 1);
+        if constexpr (S == kItems) key[k] = a.in[q].x;
+        else key[k] = places.template key<S>(q);
     }
     __syncthreads();
 #pragma unroll
@@ -365,7 +386,7 @@ __global__ void __launch_bounds__(kSortThreads, 4) k_sort_scatter(SortPass a, Pl
         if (p < here) {
             const uint32_t d = a.digit(key[k]);
             item[first[d] + seen[warp][d] + rank[k]] =
-                make_uint2(key[k], FIRST ? places.row(base + p) : a.in[base + p].y);
+                make_uint2(key[k], S == kItems ? a.in[base + p].y : places.row(base + p));
         }
     }
     __syncthreads();
@@ -412,7 +433,7 @@ struct ClusterSort {
     uint32_t count, bits, passes;
 };
 
-template <class Tok, int ITEMS>
+template <class Tok, Source S, int ITEMS>
 __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(ClusterSort a, Places<Tok> places, Clear z) {
     if (blockIdx.x >= kClusterCtas) {
         clear_rows(z, blockIdx.x - kClusterCtas, gridDim.x - kClusterCtas);
@@ -432,8 +453,8 @@ __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(ClusterSort a,
 #pragma unroll
         for (int k = 0; k < ITEMS; k++) {
             const uint32_t i = base + k * 32;
-            item[k] = make_uint2(0, 0);
-            if (i < a.count) item[k] = pass ? __ldcg(in + i) : make_uint2(places.key(i), places.row(i));
+            const uint32_t q = min(i, a.count - 1);
+            item[k] = pass ? __ldcg(in + q) : make_uint2(places.template key<S>(q), places.row(q));
         }
         for (uint32_t b = threadIdx.x; b < kWarps * kMaxBins / 2; b += kClusterThreads)
             reinterpret_cast<uint32_t*>(seen)[b] = 0;
@@ -503,13 +524,14 @@ template <class T, int V> __device__ __forceinline__ void write_row(const RunSum
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kRunThreads) k_run_sums(RunSums a, const T* __restrict__ grad, T* __restrict__ out) {
+__global__ void __launch_bounds__(kRunThreads, 3) k_run_sums(RunSums a, const T* __restrict__ grad, T* __restrict__ out) {
     __shared__ float heads[kRunThreads * V];  // [group][V * lanes]
     __shared__ uint8_t goes_on[kRunThreads];  // the group is one run, from before its first place to after its last
     const uint32_t groups = kRunThreads / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x & (a.lanes - 1);
     const uint32_t c = (blockIdx.y * a.lanes + lane) * V;
     const bool column = c < a.dim;
     const uint64_t begin = ((uint64_t)blockIdx.x * groups + group) * a.chunk;
+    const T* from = grad + (column ? c : 0);
     uint32_t cur = key_at(a, begin);
     const bool from_before = begin > 0 && cur < a.vocab && key_at(a, begin - 1) == cur;
     bool head = from_before;  // the current run is the one that came in
@@ -523,14 +545,13 @@ __global__ void __launch_bounds__(kRunThreads) k_run_sums(RunSums a, const T* __
             const uint64_t i = begin + p + k;
             const uint4 two = i < a.count ? *reinterpret_cast<const uint4*>(a.items + i) : make_uint4(0, 0, 0, 0);
             key[k] = i < a.count ? two.x : a.vocab;
-            row[k] = two.y;
+            row[k] = key[k] < a.vocab ? two.y : 0;
             key[k + 1] = i + 1 < a.count ? two.z : a.vocab;
-            row[k + 1] = two.w;
+            row[k + 1] = key[k + 1] < a.vocab ? two.w : 0;
         }
+        // a missing token's place, and a lane past the last column, read something that is not used
 #pragma unroll
-        for (int k = 0; k < kAhead; k++)
-            if (column && key[k] < a.vocab)
-                g[k] = *reinterpret_cast<const Pack<T, V>*>(grad + row[k] * a.grad_stride + c);
+        for (int k = 0; k < kAhead; k++) g[k] = *reinterpret_cast<const Pack<T, V>*>(from + row[k] * a.grad_stride);
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
             if (key[k] != cur) {
@@ -544,7 +565,7 @@ __global__ void __launch_bounds__(kRunThreads) k_run_sums(RunSums a, const T* __
                 cur = key[k];
                 acc.clear();
             }
-            if (column && key[k] < a.vocab) acc.add(g[k]);
+            acc.add(g[k]);
         }
     }
     const bool to_after = cur < a.vocab && key_at(a, begin + a.chunk) == cur;
@@ -713,12 +734,15 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
             cudaStream_t s = check_stream(stream);
             if (!n || !dim) return;
             const uint32_t v = vector_width(size, dim, table, table_stride, out, out_stride), vectors = (dim + v - 1) / v;
-            const Tokens<Tok> tk{static_cast<const Tok*>(tokens), token_row, token_col};
-            if (per_row == 1 && vectors < 1u << 30) {
-                const LookupArgs a{vocab, table_stride, n, out_stride, dim, Divisor(vectors), scale};
-                constexpr uint64_t kSpan = kLookupThreads * kLookupItems;
-                const uint64_t spans = n > (1ull << 40) / vectors ? 1u << 20 : (n * vectors + kSpan - 1) / kSpan;
-                const uint32_t blocks = (uint32_t)std::min<uint64_t>(1u << 20, spans);
+            const Tokens<Tok> tk(tokens, token_row, token_col, vocab);
+            if (per_row == 1) {
+                LookupArgs a{table_stride, n, out_stride, dim, 0, scale};
+                while (1u << a.lanes_log < lanes_for(vectors)) a.lanes_log++;
+                // every SM full once, then four rows a group, then more
+                const uint64_t wish = (n + (kLookupThreads >> a.lanes_log) - 1) / (kLookupThreads >> a.lanes_log);
+                const uint64_t full = 148 * 8;
+                const uint32_t blocks = (uint32_t)std::min<uint64_t>(
+                    1u << 20, std::max(std::min(wish, full), (wish + kLookupRows - 1) / kLookupRows));
                 with_type(type, [&](auto e) {
                     using T = decltype(e);
                     with_width<T>(v, [&](auto w) {
@@ -727,7 +751,7 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
                     });
                 });
             } else {
-                BagArgs a{vocab, table_stride, n, out_stride, dim, per_row, per_row, 0, 0, scale};
+                BagArgs a{table_stride, n, out_stride, dim, per_row, per_row, 0, 0, scale};
                 while (1u << a.lanes_log < lanes_for(vectors)) a.lanes_log++;
                 const uint32_t slices = ceil_div(vectors, 1u << a.lanes_log);
                 if (slices > kMostSlices) throw InputError("fbgpu_embed takes rows of at most 2097120 elements");
@@ -788,7 +812,7 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
             if (!vocab || !dim) return;
             char* w = static_cast<char*>(workspace);
             auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
-            const Tokens<Tok> tk{static_cast<const Tok*>(tokens), token_row, token_col};
+            const Tokens<Tok> tk(tokens, token_row, token_col, vocab);
             Clear z{static_cast<char*>(out), vocab, (uint64_t)dim * size, out_stride * size};
             if (out_stride == dim) z = Clear{z.p, 1, vocab * z.bytes, 0};
             const uint64_t cleared = z.rows * ((z.bytes + 15) / 16);
@@ -800,8 +824,8 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
                 FB_CUDA_CHECK(cudaGetLastError());
                 return;
             }
-            const Places<Tok> places{tk, Divisor(per_row), vocab,
-                                     (per_row == 1 || token_col == 1) && (n == 1 || token_row == per_row)};
+            const Places<Tok> places{tk, Divisor(per_row)};
+            const bool flat = (per_row == 1 || token_col == 1) && (n == 1 || token_row == per_row);
             uint2* items[2] = {reinterpret_cast<uint2*>(w + ws.items[0]), reinterpret_cast<uint2*>(w + ws.items[1])};
             if (ws.count <= kClusterPlaces) {
                 const ClusterSort a{{items[0], items[1]}, ws.count, ws.bits, ws.passes};
@@ -818,7 +842,10 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
                     cfg.attrs = &attr;
                     cfg.numAttrs = 1;
                     count_launch();
-                    FB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sort_cluster<Tok, decltype(of)::value>, a, places, z));
+                    if (flat)
+                        FB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sort_cluster<Tok, kFlat, decltype(of)::value>, a, places, z));
+                    else
+                        FB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sort_cluster<Tok, kStrided, decltype(of)::value>, a, places, z));
                 };
                 const uint32_t each = ceil_div(ws.count, kClusterCtas * kClusterThreads);  // places of a thread
                 if (each <= 2) launch(std::integral_constant<int, 2>{});
@@ -837,15 +864,15 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
                     a.shift = p * ws.bits;
                     a.bits = ws.bits;
                     for (int k = 0; k < 3; k++) count_launch();
-                    if (p == 0) {
-                        k_sort_count<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
+                    auto pass = [&](auto source) {
+                        constexpr Source S = decltype(source)::value;
+                        k_sort_count<Tok, S><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
                         k_sort_scan<<<1u << ws.bits, kSortThreads, 0, s>>>(a);
-                        k_sort_scatter<Tok, true><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
-                    } else {
-                        k_sort_count<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
-                        k_sort_scan<<<1u << ws.bits, kSortThreads, 0, s>>>(a);
-                        k_sort_scatter<Tok, false><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
-                    }
+                        k_sort_scatter<Tok, S><<<ws.tiles, kSortThreads, 0, s>>>(a, places);
+                    };
+                    if (p) pass(std::integral_constant<Source, kItems>{});
+                    else if (flat) pass(std::integral_constant<Source, kFlat>{});
+                    else pass(std::integral_constant<Source, kStrided>{});
                 }
             }
             const int last = (ws.passes - 1) & 1;
