@@ -20,10 +20,9 @@
 namespace fbg {
 namespace {
 
-constexpr uint32_t kMostSlices = 65535;  // of columns: a grid's y extent
+__global__ void __launch_bounds__(256) k_clear(Clear z) { clear_rows(z, blockIdx.x, gridDim.x); }
 
-// What a missing token's lookup reads.
-__device__ __align__(16) const uint4 g_zero{0, 0, 0, 0};
+constexpr uint32_t kMostSlices = 65535;  // of columns: a grid's y extent
 
 template <class Tok> struct Tokens {
     // Tokens as unsigned numbers of their own width: a negative one is above every `vocab`, which is at most
@@ -36,20 +35,6 @@ template <class Tok> struct Tokens {
         : p(static_cast<const Tok*>(p_)), row(row_), col(col_),
           vocab((U)std::min<uint64_t>(vocab_, 1ull << (8 * sizeof(Tok) - 1))) {}
     __device__ __forceinline__ U at(uint64_t r, uint64_t j) const { return (U)p[r * row + j * col]; }
-};
-
-// i / d for i < 2^31: with l = ceil(log2 d), floor(i * (floor(2^(31+l) / d) + 1) / 2^(31+l)), as the excess of the
-// multiplier over 2^(31+l) / d, at most 1, times i stays below 2^31 and so below a unit of the quotient.
-struct Divisor {
-    uint32_t d, mul, shift;
-    explicit Divisor(uint32_t d_ = 1) : d(d_), mul(0), shift(0) {
-        if (d <= 1) return;
-        uint32_t l = 0;
-        while ((1ull << l) < d) l++;
-        mul = (uint32_t)((1ull << (31 + l)) / d + 1);
-        shift = l - 1;
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t i) const { return d <= 1 ? i : __umulhi(i, mul) >> shift; }
 };
 
 // A vector of f32 sums.  Pairs are added by one instruction (add.rn.f32x2), each
@@ -404,30 +389,6 @@ __global__ void __launch_bounds__(kSortThreads, 4) k_sort_scatter(SortPass a, Pl
 constexpr int kClusterThreads = 512, kClusterCtas = 8;
 constexpr uint32_t kClusterPlaces = kClusterCtas * kClusterThreads * 16;
 
-struct Clear {
-    char* p;          // rows of `bytes` bytes, `stride` bytes apart
-    uint64_t rows, bytes, stride;
-};
-
-// Block `b` of `blocks` clears its share.
-__device__ __forceinline__ void clear_rows(const Clear& z, uint64_t b, uint64_t blocks) {
-    const uint64_t per = 16ull * blockDim.x;  // bytes of a block's step
-    const uint64_t steps = (z.bytes + 15 + per - 1) / per;
-    for (uint64_t i = b; i < z.rows * steps; i += blocks) {
-        const uint64_t r = z.rows == 1 ? 0 : i / steps;
-        char* row = z.p + r * z.stride;
-        char* end = row + z.bytes;
-        char* at = reinterpret_cast<char*>((uintptr_t)row & ~(uintptr_t)15) + (i - r * steps) * per + 16 * threadIdx.x;
-        if (at >= row && at + 16 <= end) {
-            *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
-        } else {  // elements are two or four bytes
-            for (int k = 0; k < 16; k += 2)
-                if (at + k >= row && at + k < end) *reinterpret_cast<uint16_t*>(at + k) = 0;
-        }
-    }
-}
-__global__ void __launch_bounds__(256) k_clear(Clear z) { clear_rows(z, blockIdx.x, gridDim.x); }
-
 struct ClusterSort {
     uint2* items[2];  // pass p writes set p & 1
     uint32_t count, bits, passes;
@@ -713,6 +674,14 @@ bool grad_sizes_fit(uint64_t n, uint64_t per_row, uint64_t vocab) {
 }
 
 }  // namespace
+
+void launch_clear(void* p, uint64_t rows, uint64_t bytes, uint64_t stride, cudaStream_t s) {
+    const Clear z = clear_of(p, rows, bytes, stride);
+    const uint64_t units = z.rows * ((z.bytes + 15) / 16);
+    count_launch();
+    k_clear<<<(uint32_t)std::min<uint64_t>(148 * 8, (units + 255) / 256), 256, 0, s>>>(z);
+}
+
 }  // namespace fbg
 
 extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vocab, uint32_t dim,
@@ -813,13 +782,10 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
             char* w = static_cast<char*>(workspace);
             auto at = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
             const Tokens<Tok> tk(tokens, token_row, token_col, vocab);
-            Clear z{static_cast<char*>(out), vocab, (uint64_t)dim * size, out_stride * size};
-            if (out_stride == dim) z = Clear{z.p, 1, vocab * z.bytes, 0};
+            const Clear z = clear_of(out, vocab, (uint64_t)dim * size, out_stride * size);
             const uint64_t cleared = z.rows * ((z.bytes + 15) / 16);
-            if (ws.count == 0 || ws.count > kClusterPlaces) {
-                count_launch();
-                k_clear<<<(uint32_t)std::min<uint64_t>(148 * 8, (cleared + 255) / 256), 256, 0, s>>>(z);
-            }
+            if (ws.count == 0 || ws.count > kClusterPlaces)
+                launch_clear(out, vocab, (uint64_t)dim * size, out_stride * size, s);
             if (ws.count == 0) {
                 FB_CUDA_CHECK(cudaGetLastError());
                 return;

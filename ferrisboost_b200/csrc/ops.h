@@ -28,6 +28,53 @@ __device__ __host__ __forceinline__ uint64_t mix64(uint64_t z) {
     return z ^ (z >> 31);
 }
 
+// What is read in place of something that is not there.
+static __device__ __align__(16) const uint4 g_zero{0, 0, 0, 0};
+
+// i / d for i < 2^31: with l = ceil(log2 d), floor(i * (floor(2^(31+l) / d) + 1) / 2^(31+l)), as the excess of the
+// multiplier over 2^(31+l) / d, at most 1, times i stays below 2^31 and so below a unit of the quotient.
+struct Divisor {
+    uint32_t d, mul, shift;
+    Divisor(uint32_t d_ = 1) : d(d_), mul(0), shift(0) {
+        if (d <= 1) return;
+        uint32_t l = 0;
+        while ((1ull << l) < d) l++;
+        mul = (uint32_t)((1ull << (31 + l)) / d + 1);
+        shift = l - 1;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t i) const { return d <= 1 ? i : __umulhi(i, mul) >> shift; }
+};
+
+struct Clear {
+    char* p;          // rows of `bytes` bytes, `stride` bytes apart
+    uint64_t rows, bytes, stride;
+};
+
+// Rows that follow one another are one.
+inline Clear clear_of(void* p, uint64_t rows, uint64_t bytes, uint64_t stride) {
+    if (stride == bytes) return Clear{static_cast<char*>(p), 1, rows * bytes, 0};
+    return Clear{static_cast<char*>(p), rows, bytes, stride};
+}
+void launch_clear(void* p, uint64_t rows, uint64_t bytes, uint64_t stride, cudaStream_t s);  // embed.cu
+
+// Block `b` of `blocks` clears its share.
+__device__ __forceinline__ void clear_rows(const Clear& z, uint64_t b, uint64_t blocks) {
+    const uint64_t per = 16ull * blockDim.x;  // bytes of a block's step
+    const uint64_t steps = (z.bytes + 15 + per - 1) / per;
+    for (uint64_t i = b; i < z.rows * steps; i += blocks) {
+        const uint64_t r = z.rows == 1 ? 0 : i / steps;
+        char* row = z.p + r * z.stride;
+        char* end = row + z.bytes;
+        char* at = reinterpret_cast<char*>((uintptr_t)row & ~(uintptr_t)15) + (i - r * steps) * per + 16 * threadIdx.x;
+        if (at >= row && at + 16 <= end) {
+            *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+        } else {  // elements are two or four bytes
+            for (int k = 0; k < 16; k += 2)
+                if (at + k >= row && at + k < end) *reinterpret_cast<uint16_t*>(at + k) = 0;
+        }
+    }
+}
+
 // Runs f with a value of the element type `type` names.
 template <class F> void with_type(int32_t type, F&& f) {
     switch (type) {
