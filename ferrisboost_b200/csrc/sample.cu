@@ -33,7 +33,7 @@ __device__ __forceinline__ Limits limits_of(const fbgpu_sample_params& p, uint64
     const float tp = p.top_ps ? p.top_ps[r] : p.top_p;
     const float mp = p.min_ps ? p.min_ps[r] : p.min_p;
     l.greedy = !(t > 0.0f);
-    l.inv_t = l.greedy ? 0.0f : __fdiv_rn(1.0f, fminf(t, FLT_MAX));  // never 0: no 0 * infinity in exp_of
+    l.inv_t = l.greedy ? 0.0f : __fdiv_rn(1.0f, fminf(fmaxf(t, FLT_MIN), FLT_MAX));  // neither 0 nor infinite
     l.top_k = k < 1 || (uint32_t)k > classes ? classes : (uint32_t)k;
     l.use_p = tp < 1.0f;
     l.top_p = tp > 0.0f ? (double)tp : 0.0;
@@ -51,9 +51,9 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float score_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
+// `top` is finite (see the two kernels for a maximum of +infinity).
 __device__ __forceinline__ float exp_of(float x, float top, float inv_t) {
-    if (x == top) return 1.0f;
-    return x == -INFINITY || top == INFINITY ? 0.0f : expf(__fmul_rn(__fsub_rn(x, top), inv_t));
+    return expf(__fmul_rn(__fsub_rn(x, top), inv_t));
 }
 // exp * 2^40 is exact; what is below 2^-40 of the maximum weighs nothing.
 __device__ __forceinline__ u64 weight_of(float e) { return __float2ull_rz(__fmul_rn(e, 1099511627776.0f)); }
@@ -95,6 +95,11 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
                 if (x[i] == top) drawn = i;
             share = 1.0f;
         } else if (top > -INFINITY) {
+            if (top == INFINITY) {  // only the infinite ones weigh
+#pragma unroll
+                for (int i = 0; i < KP; i++) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+                top = 0.0f;
+            }
             u64 w[KP];
             uint32_t keep = 0;
 #pragma unroll
@@ -103,29 +108,36 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
                 w[i] = weight_of(e);
                 if (!(e < l.min_p)) keep |= 1u << i;
             }
-            if (l.top_k < classes || l.use_p) {
-                u64 sum = 0;
-                uint32_t first = 0;  // the top_k first
+            u64 sum = 0;
+            if (l.top_k < classes) {
 #pragma unroll
                 for (int i = 0; i < KP; i++) {
                     uint32_t rank = 0;
 #pragma unroll
                     for (int j = 0; j < KP; j++)
                         if (j != i) rank += j < i ? x[j] >= x[i] : x[j] > x[i];
-                    if (rank < l.top_k) first |= 1u << i, sum += w[i];
+                    if (rank >= l.top_k) keep &= ~(1u << i);
+                    else sum += w[i];
                 }
-                keep &= first;
-                if (l.use_p) {
-                    const u64 goal = goal_of(l.top_p, sum);
+            } else if (l.use_p) {
 #pragma unroll
-                    for (int i = 0; i < KP; i++) {
-                        u64 before = 0;
+                for (int i = 0; i < KP; i++) sum += w[i];
+            }
+            if (l.use_p) {
+                const u64 goal = goal_of(l.top_p, sum);
+                u64 before[KP] = {};  // the weight of the classes in front of each
 #pragma unroll
-                        for (int j = 0; j < KP; j++)
-                            if (j != i && (j < i ? x[j] >= x[i] : x[j] > x[i])) before += w[j];
-                        if (before >= goal) keep &= ~(1u << i);
+                for (int i = 0; i < KP; i++) {
+#pragma unroll
+                    for (int j = i + 1; j < KP; j++) {
+                        const bool later = x[j] > x[i];  // the later class comes first
+                        if (later) before[i] += w[j];
+                        else before[j] += w[i];
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < KP; i++)
+                    if (before[i] >= goal) keep &= ~(1u << i);
             }
             u64 total = 0;
 #pragma unroll
@@ -145,42 +157,51 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
 }
 
 // ------------------------------------------- a warp, block or cluster per row
-// WARPS warps of CTAS blocks (one cluster) hold a row.  Warp after warp takes a
-// contiguous part of it; within the part, lane after lane takes VEC elements a
-// step.  NV steps are kept in registers; NV = 0 reads the row again for every
-// step.  Vectors are aligned in memory, not in the row: a row that starts off a
-// 16-byte boundary has `shift` places before its first class, which are masked.
-template <int WARPS, int CTAS> struct RowShared {
+// WARPS warps of CTAS blocks (one cluster) hold a row.  Its scores are brought
+// into shared memory as f32 once (HELD; a row too long for that is read again
+// for every step) and every later step is a short loop over them: held in
+// registers, the unrolled steps ran out of the instruction cache.  Places are
+// counted from the 16-byte boundary at or before the row's first class, so that
+// the loads are aligned vectors; the places before that class, and after the
+// last, hold -infinity.  Block after block, and in it warp after warp, takes
+// a contiguous part of the places; a step is four of a lane.
+constexpr int kSort = 1024;  // the most classes that are sorted
+
+template <int WARPS, int CTAS> struct alignas(16) RowShared {
     static constexpr int kBins = WARPS == 1 ? 256 : 1024;
     static constexpr int kList = WARPS == 1 ? 64 : 128;
+    static constexpr int kSorted = WARPS == 1 ? 1 : kSort;
     uint32_t low[kBins], high[kBins];     // a bin's count, or its weight as two words
     u64 part[2][WARPS];                   // warps' partial sums; two sets, used in turn
-    uint32_t found[2];                    // members of the chosen bin
+    uint32_t found[3];                    // members of the chosen bin; of the list to sort
     uint32_t key[2][kList], all_key[kList];
     u64 weight[2][kList], all_weight[kList];
     u64 scan[WARPS];
-    uint32_t bin;
     u64 before, pick_above;
-    uint32_t pick_key, pick_same;
+    uint32_t bin, pick_key, pick_same;
+    u64 sorted[kSorted], sorted_weight[kSorted];
 };
 
-template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
+template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     using Sh = RowShared<WARPS, CTAS>;
-    static constexpr int kSets = NV ? NV : 1;
-    static constexpr int kBins = Sh::kBins;
-    static constexpr int kThreadsPerRow = WARPS * 32;
+    static constexpr int kBins = Sh::kBins, kThreads = WARPS * 32, kStep = 128;
 
     Sh& s;
+    float* x;             // HELD: the block's places
     const T* row;
-    uint32_t classes, shift, first, steps;  // the part's first place (with shift), and its steps
+    uint32_t classes, shift;
+    uint32_t steps;       // of a warp
+    uint32_t block_first, warp_first;  // first places
     int lane, warp, tid, cta, parity = 0;
-    Pack<T, VEC> held[kSets];
+    float most;           // HELD: the largest score that this thread brought
 
-    __device__ __forceinline__ RowDraw(Sh& sh) : s(sh) {
+    __device__ __forceinline__ RowDraw(Sh& sh, float* held, uint32_t steps_) : s(sh), x(held), steps(steps_) {
         lane = threadIdx.x & 31;
         warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
         tid = WARPS == 1 ? lane : threadIdx.x;
         cta = CTAS == 1 ? 0 : (int)cooperative_groups::this_cluster().block_rank();
+        block_first = cta * WARPS * steps * kStep;
+        warp_first = block_first + warp * steps * kStep;
     }
 
     __device__ __forceinline__ void sync_block() {
@@ -196,62 +217,76 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
         if (CTAS == 1) return p;
         return cooperative_groups::this_cluster().map_shared_rank(p, c);
     }
-
-    __device__ __forceinline__ Pack<T, VEC> read(uint32_t v) {
-        const uint32_t place = first + (v * 32 + lane) * VEC;
-        Pack<T, VEC> p;
-        if (VEC > 1 && place >= shift && place + VEC <= shift + classes) {
-            p = *reinterpret_cast<const Pack<T, VEC>*>(row + (place - shift));
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; i++)
-                p.v[i] = place + i >= shift && place + i < shift + classes ? row[place + i - shift]
-                                                                           : from_f32<T>(-INFINITY);
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; i++) p.v[i] = from_f32<T>(score(to_f32(p.v[i])));
-        return p;
+    __device__ __forceinline__ float one(uint32_t place) {
+        return place >= shift && place < shift + classes ? score(to_f32(row[place - shift])) : -INFINITY;
     }
+
     __device__ __forceinline__ void open(const T* row_, uint32_t classes_) {
+        constexpr int V = 16 / sizeof(T), kAhead = 4;
         row = row_;
         classes = classes_;
-        shift = VEC > 1 ? (uint32_t)(((uintptr_t)row % (VEC * sizeof(T))) / sizeof(T)) : 0;
-        const uint32_t vectors = (classes + shift + VEC - 1) / VEC;
-        steps = NV ? NV : (vectors + 32 * WARPS * CTAS - 1) / (32 * WARPS * CTAS);
-        first = (cta * WARPS + warp) * steps * 32 * VEC;
-        if constexpr (NV > 0) {
+        shift = (uint32_t)(((uintptr_t)row % 16) / sizeof(T));
+        if (!HELD) return;
+        most = -INFINITY;
+        sync_block();  // the row before is no longer read
+        const uint32_t vectors = WARPS * steps * kStep / V;
+        for (uint32_t v0 = tid; v0 < vectors; v0 += kAhead * kThreads) {
+            union {
+                uint4 u;
+                T v[V];
+            } p[kAhead];
+            bool whole[kAhead];
 #pragma unroll
-            for (int v = 0; v < NV; v++) held[v] = read(v);
-        }
-    }
-    // f(score, step, index within the vector) for each of the lane's places
-    template <class F> __device__ __forceinline__ void each(F&& f) {
-        if constexpr (NV > 0) {
-#pragma unroll
-            for (int v = 0; v < NV; v++) {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) f(to_f32(held[v].v[i]));
+            for (int k = 0; k < kAhead; k++) {
+                const uint32_t place = block_first + (v0 + k * kThreads) * V;
+                whole[k] = place >= shift && place + V <= shift + classes;
+                p[k].u = *(whole[k] ? reinterpret_cast<const uint4*>(row + (place - shift)) : &g_zero);
             }
-        } else {
-            for (uint32_t v = 0; v < steps; v++) {
-                const Pack<T, VEC> p = read(v);
 #pragma unroll
-                for (int i = 0; i < VEC; i++) f(to_f32(p.v[i]));
+            for (int k = 0; k < kAhead; k++) {
+                const uint32_t v = v0 + k * kThreads, place = block_first + v * V;
+                if (v >= vectors) break;
+                float f[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) f[i] = score(to_f32(p[k].v[i]));
+                if (!whole[k]) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) f[i] = one(place + i);
+                }
+#pragma unroll
+                for (int i = 0; i < V; i++) most = fmaxf(most, f[i]);
+#pragma unroll
+                for (int i = 0; i < V; i += 4)
+                    *reinterpret_cast<float4*>(x + v * V + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
             }
         }
+        sync_block();
     }
-    // f(scores of a step, the place of the first) step by step, in order
+    // f(scores, place of the first) for each of the lane's steps, in order
     template <class F> __device__ __forceinline__ void each_step(F&& f) {
-        if constexpr (NV > 0) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < steps; i++) {
+            const uint32_t place = warp_first + i * kStep + lane * 4;
+            Pack<float, 4> p;
+            if (HELD) {
+                p = *reinterpret_cast<const Pack<float, 4>*>(x + (place - block_first));
+            } else {
 #pragma unroll
-            for (int v = 0; v < NV; v++) f(held[v], first + (v * 32 + lane) * VEC);
-        } else {
-            for (uint32_t v = 0; v < steps; v++) f(read(v), first + (v * 32 + lane) * VEC);
+                for (int k = 0; k < 4; k++) p.v[k] = one(place + k);
+            }
+            f(p, place);
         }
+    }
+    // f(score) for each of the lane's places
+    template <class F> __device__ __forceinline__ void each(F&& f) {
+        each_step([&](const Pack<float, 4>& p, uint32_t) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) f(p.v[k]);
+        });
     }
 
     // A reduction over the row's threads; op is commutative.  `before` gets the
-    // result over the warps in front of this one (for sums).
+    // result over the warps in front of this one.
     template <class Op> __device__ __forceinline__ u64 reduce(u64 v, u64 zero, Op&& op, u64* before = nullptr) {
 #pragma unroll
         for (int d = 16; d; d /= 2) v = op(v, (u64)__shfl_xor_sync(0xffffffffu, v, d));
@@ -259,37 +294,168 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
         if (WARPS == 1) return v;
         if (lane == 0) s.part[parity][warp] = v;
         sync_row();
-        u64 all = zero;
-        for (int c = 0; c < CTAS; c++) {
-            const u64* p = at(s.part[parity], c);
-            // lane w takes warp w's value
-            u64 x = lane < WARPS ? p[lane] : zero;
-            if (before) {
-                u64 y = c < cta || (c == cta && lane < warp) ? x : zero;
+        u64 all = zero, front = zero;
 #pragma unroll
-                for (int d = 16; d; d /= 2) y = op(y, (u64)__shfl_xor_sync(0xffffffffu, y, d));
-                *before = op(*before, y);
-            }
-            all = op(all, x);
+        for (int c = 0; c < CTAS; c++) {
+            // lane w takes warp w's value
+            const u64 y = lane < WARPS ? at(s.part[parity], c)[lane] : zero;
+            all = op(all, y);
+            if (c < cta || (c == cta && lane < warp)) front = op(front, y);
         }
 #pragma unroll
-        for (int d = 16; d; d /= 2) all = op(all, (u64)__shfl_xor_sync(0xffffffffu, all, d));
+        for (int d = 16; d; d /= 2) {
+            all = op(all, (u64)__shfl_xor_sync(0xffffffffu, all, d));
+            if (before) front = op(front, (u64)__shfl_xor_sync(0xffffffffu, front, d));
+        }
+        if (before) *before = front;
         parity ^= 1;
         return all;
     }
     __device__ __forceinline__ u64 sum(u64 v, u64* before = nullptr) {
         return reduce(v, 0, [](u64 a, u64 b) { return a + b; }, before);
     }
-
-    __device__ __forceinline__ uint32_t bin_of(float x, float top, float per) {
-        return min((uint32_t)(kBins - 1), __float2uint_rz(__fmul_rn(__fsub_rn(top, x), per)));
+    // Over the block's threads: the sum in front of this one, and the total.
+    __device__ __forceinline__ u64 block_before(u64 mine, u64& total) {
+        u64 upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const u64 y = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += y;
+        }
+        total = __shfl_sync(0xffffffffu, upto, 31);
+        if (WARPS > 1) {
+            sync_block();
+            if (lane == 31) s.scan[warp] = upto;
+            sync_block();
+            u64 all = lane < WARPS ? s.scan[lane] : 0, front = lane < warp ? all : 0;
+#pragma unroll
+            for (int d = 16; d; d /= 2) {
+                all += __shfl_xor_sync(0xffffffffu, all, d);
+                front += __shfl_xor_sync(0xffffffffu, front, d);
+            }
+            total = all;
+            upto += front;
+        }
+        return upto - mine;
     }
 
-    __device__ void draw(uint64_t r, const fbgpu_sample_params& params, const float* u, int32_t* out_classes,
-                         float* out_probs) {
+    __device__ __forceinline__ uint32_t bin_of(float v, float top, float per) {
+        return min((uint32_t)(kBins - 1), __float2uint_rz(__fmul_rn(__fsub_rn(top, v), per)));
+    }
+    __device__ __forceinline__ void clear_bins(int set) {
+        for (int i = tid; i < kBins; i += kThreads) s.low[i] = s.high[i] = 0;
+        if (tid == 0) s.found[set] = 0, s.bin = kBins;
+        sync_block();
+    }
+    // After the bins are filled: the bin in which the running sum reaches the goal that goal_for(total) names
+    // (kBins: none), and the sum before it.  Every block of a cluster does the same work.
+    template <class G> __device__ __forceinline__ uint32_t find_bin(u64& before, u64& goal, G&& goal_for) {
+        constexpr int kPer = kBins / kThreads;
+        sync_row();
+        u64 v[kPer], mine = 0, total;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            v[i] = 0;
+#pragma unroll
+            for (int c = 0; c < CTAS; c++)
+                v[i] += (u64)at(s.high, c)[tid * kPer + i] << 32 | at(s.low, c)[tid * kPer + i];
+            mine += v[i];
+        }
+        u64 run = block_before(mine, total);
+        goal = goal_for(total);
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            if (run < goal && goal <= run + v[i]) {
+                s.bin = tid * kPer + i;
+                s.before = run;
+            }
+            run += v[i];
+        }
+        sync_block();
+        before = s.before;
+        return s.bin;
+    }
+
+    // Bitonic, falling, of a power of two of items.
+    __device__ __forceinline__ void sort(u64* a, uint32_t count) {
+        for (uint32_t k = 2; k <= count; k *= 2) {
+            for (uint32_t j = k / 2; j; j /= 2) {
+                for (uint32_t i = tid; i < count / 2; i += kThreads) {
+                    const uint32_t lo = (i & ~(j - 1)) << 1 | (i & (j - 1)), hi = lo | j;
+                    const u64 u = a[lo], v = a[hi];
+                    if ((u < v) == ((lo & k) == 0)) a[lo] = v, a[hi] = u;
+                }
+                sync_block();
+            }
+        }
+    }
+
+    // The draw from a sorted list of the row's first `members` classes, by one block; the limits end inside it.
+    __device__ __forceinline__ void draw_sorted(uint32_t members, uint64_t r, const Limits& l, float top, float u,
+                                                int32_t* out_classes, float* out_probs) {
+        constexpr int kPer = kSort / kThreads;
+        uint32_t count = 32;
+        while (count < members) count *= 2;
+        for (uint32_t i = members + tid; i < count; i += kThreads) s.sorted[i] = 0;
+        sync_block();
+        sort(s.sorted, count);
+        u64 item[kPer], w[kPer], mine = 0, total;
+        float e[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const uint32_t rank = tid * kPer + i;
+            item[i] = rank < members && rank < l.top_k ? s.sorted[rank] : 0;
+            e[i] = item[i] ? exp_of(score_of((uint32_t)(item[i] >> 32)), top, l.inv_t) : 0.0f;
+            w[i] = weight_of(e[i]);
+            mine += w[i];
+        }
+        u64 before = block_before(mine, total);
+        const u64 goal = l.use_p ? goal_of(l.top_p, total) : ~0ull;
+        mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const uint32_t rank = tid * kPer + i;
+            const bool keep = item[i] && before < goal && !(e[i] < l.min_p);
+            before += w[i];
+            if (!keep) w[i] = 0;
+            mine += w[i];
+            // to be ordered by class: the low word is the class's complement
+            if (rank < count) {
+                s.sorted_weight[rank] = w[i];
+                s.sorted[rank] = keep ? item[i] << 32 | rank : 0;
+            }
+        }
+        block_before(mine, total);
+        uint32_t kept = 32;
+        while (kept < members && kept < l.top_k) kept *= 2;
+        sync_block();
+        sort(s.sorted, kept);
+        mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const uint32_t q = tid * kPer + i;
+            item[i] = q < kept ? s.sorted[q] : 0;
+            w[i] = item[i] ? s.sorted_weight[(uint32_t)item[i]] : 0;
+            mine += w[i];
+        }
+        u64 all, run = block_before(mine, all);
+        const u64 place = place_of(u, total);
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            if (place >= run && place < run + w[i]) {
+                out_classes[r] = (int32_t)~(uint32_t)(item[i] >> 32);
+                if (out_probs) out_probs[r] = share_of(w[i], total);
+            }
+            run += w[i];
+        }
+    }
+
+    __device__ __forceinline__ void draw(uint64_t r, const fbgpu_sample_params& params, const float* u,
+                                         int32_t* out_classes, float* out_probs) {
         const Limits l = limits_of(params, r, classes);
         float top = -INFINITY;
-        each([&](float x) { top = fmaxf(top, x); });
+        if (HELD) top = most;
+        else each([&](float v) { top = fmaxf(top, v); });
         {
             const uint32_t k = (uint32_t)reduce(key_of(top), 0, [](u64 a, u64 b) { return a > b ? a : b; });
             top = score_of(k);
@@ -301,6 +467,50 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
             }
             return;
         }
+        const bool certain = top == INFINITY;  // only the infinite ones weigh
+        if (certain) top = FLT_MAX;
+        // Scores as they count: +infinity as FLT_MAX, and then everything else as -infinity.
+        auto seen = [&](float v) { return certain ? (v == INFINITY ? FLT_MAX : -INFINITY) : v; };
+        // Weights vanish 27.73 T below the maximum: bins over that span, falling, the last for the rest.
+        const float per = __fmul_rn(kBins / 27.75f, l.inv_t);
+        if (WARPS > 1 && !l.greedy && l.top_k < classes && l.top_k <= kSort) {
+            // At least top_k classes are at or above the top_k-th largest of the threads' maxima: those are sorted.
+            clear_bins(2);
+            if (HELD && l.top_k * 4 <= kThreads * CTAS) {
+                if (seen(most) > -INFINITY) atomicAdd(&s.low[bin_of(seen(most), top, per)], 1u);
+            } else {
+                each([&](float v) {
+                    if (seen(v) > -INFINITY) atomicAdd(&s.low[bin_of(seen(v), top, per)], 1u);
+                });
+            }
+            u64 before, goal;
+            const uint32_t bin = find_bin(before, goal, [&](u64) { return (u64)l.top_k; });
+            each_step([&](const Pack<float, 4>& p, uint32_t place) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float v = seen(p.v[i]);
+                    if (v > -INFINITY && bin_of(v, top, per) <= bin) {
+                        const uint32_t q = atomicAdd(&s.found[2], 1u);
+                        if (q < kSort) s.sorted[q] = (u64)key_of(v) << 32 | ~(place + i - shift);
+                    }
+                }
+            });
+            sync_row();
+            uint32_t members = 0;
+            for (int c = 0; c < CTAS; c++) members += *at(&s.found[2], c);
+            if (members <= kSort) {
+                if (cta == 0) {
+                    uint32_t base = s.found[2];
+                    for (int c = 1; c < CTAS; c++) {
+                        const uint32_t m = *at(&s.found[2], c);
+                        for (uint32_t i = tid; i < m; i += kThreads) s.sorted[base + i] = at(s.sorted, c)[i];
+                        base += m;
+                    }
+                    draw_sorted(members, r, l, top, u[r], out_classes, out_probs);
+                }
+                return;
+            }
+        }
         // kept: key > cut, or key == cut and one of the first `ties` of the `same` classes of that key
         uint32_t cut = 0, ties = 0xffffffffu, same = 0;
         if (l.greedy) {
@@ -308,19 +518,17 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
             ties = 1;
             same = 0xffffffffu;
         } else {
-            // Weights vanish 27.73 T below the maximum: bins over that span, falling, the last for the rest.
-            const float per = __fmul_rn(kBins / 27.75f, l.inv_t);
             // first by count for top_k, then by weight for top_p
+#pragma unroll 1
             for (int by_weight = 0; by_weight < 2; by_weight++) {
                 if (by_weight ? !l.use_p : l.top_k >= classes) continue;
-                for (int i = tid; i < kBins; i += kThreadsPerRow) s.low[i] = s.high[i] = 0;
-                if (tid == 0) s.found[by_weight] = 0;
-                sync_block();
-                each([&](float x) {
-                    if (x == -INFINITY || key_of(x) < cut) return;
-                    const uint32_t b = bin_of(x, top, per);
+                clear_bins(by_weight);
+                each([&](float v) {
+                    v = seen(v);
+                    if (v == -INFINITY || key_of(v) < cut) return;
+                    const uint32_t b = bin_of(v, top, per);
                     if (by_weight) {
-                        const u64 w = weight_of(exp_of(x, top, l.inv_t));
+                        const u64 w = weight_of(exp_of(v, top, l.inv_t));
                         if (w == 0) return;
                         const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.low[b], lo);
                         const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < lo);
@@ -329,71 +537,28 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
                         atomicAdd(&s.low[b], 1u);
                     }
                 });
-                sync_row();
-                // each thread: the running sum before its bins (every block of a cluster does the same work)
-                constexpr int kPer = kBins / kThreadsPerRow;
-                u64 v[kPer], mine = 0;
-#pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    v[i] = 0;
-                    for (int c = 0; c < CTAS; c++)
-                        v[i] += (u64)at(s.high, c)[tid * kPer + i] << 32 | at(s.low, c)[tid * kPer + i];
-                    mine += v[i];
-                }
-                u64 upto = mine;
-#pragma unroll
-                for (int d = 1; d < 32; d *= 2) {
-                    const u64 y = __shfl_up_sync(0xffffffffu, upto, d);
-                    if (lane >= d) upto += y;
-                }
-                u64 total = __shfl_sync(0xffffffffu, upto, 31);
-                if (WARPS > 1) {
-                    if (lane == 31) s.scan[warp] = upto;
-                    if (tid == 0) s.bin = kBins;
-                    sync_block();
-                    u64 x = lane < WARPS ? s.scan[lane] : 0, y = lane < warp ? x : 0;
-#pragma unroll
-                    for (int d = 16; d; d /= 2) {
-                        x += __shfl_xor_sync(0xffffffffu, x, d);
-                        y += __shfl_xor_sync(0xffffffffu, y, d);
-                    }
-                    total = x;
-                    upto += y;
-                } else if (tid == 0) {
-                    s.bin = kBins;
-                }
-                u64 goal = l.top_k;
-                if (by_weight) {
+                u64 before, goal;
+                const uint32_t bin = find_bin(before, goal, [&](u64 total) -> u64 {
+                    if (!by_weight) return l.top_k;
                     if (ties < same) total -= (same - ties) * weight_of(exp_of(score_of(cut), top, l.inv_t));
-                    goal = goal_of(l.top_p, total);
-                }
-                sync_block();
-                u64 run = upto - mine;
-#pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    if (run < goal && goal <= run + v[i]) {
-                        s.bin = tid * kPer + i;
-                        s.before = run;
-                    }
-                    run += v[i];
-                }
-                sync_block();
-                const uint32_t bin = s.bin;
+                    return goal_of(l.top_p, total);
+                });
                 if (bin == kBins) {  // the whole row stays below the goal
                     if (CTAS > 1) sync_row();  // the other blocks may still read these bins
                     continue;
                 }
-                goal -= s.before;
+                goal -= before;
                 // the chosen bin's members
-                auto member = [&](float x) {
-                    return x > -INFINITY && key_of(x) >= cut && bin_of(x, top, per) == bin;
+                auto member = [&](float v) {
+                    return v > -INFINITY && key_of(v) >= cut && bin_of(v, top, per) == bin;
                 };
-                each([&](float x) {
-                    if (!member(x)) return;
+                each([&](float v) {
+                    v = seen(v);
+                    if (!member(v)) return;
                     const uint32_t q = atomicAdd(&s.found[by_weight], 1u);
                     if (q < Sh::kList) {
-                        s.key[by_weight][q] = key_of(x);
-                        s.weight[by_weight][q] = by_weight ? weight_of(exp_of(x, top, l.inv_t)) : 1;
+                        s.key[by_weight][q] = key_of(v);
+                        s.weight[by_weight][q] = by_weight ? weight_of(exp_of(v, top, l.inv_t)) : 1;
                     }
                 });
                 sync_row();
@@ -407,7 +572,7 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
                         uint32_t base = 0;
                         for (int c = 0; c < CTAS; c++) {
                             const uint32_t m = *at(&s.found[by_weight], c);
-                            for (uint32_t i = tid; i < m; i += kThreadsPerRow) {
+                            for (uint32_t i = tid; i < m; i += kThreads) {
                                 s.all_key[base + i] = at(s.key[by_weight], c)[i];
                                 s.all_weight[base + i] = at(s.weight[by_weight], c)[i];
                             }
@@ -417,18 +582,18 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
                         weights = s.all_weight;
                         sync_block();
                     }
-                    for (uint32_t i = tid; i < members; i += kThreadsPerRow) {
+                    for (uint32_t i = tid; i < members; i += kThreads) {
                         const uint32_t key = keys[i];
-                        u64 before = 0;
+                        u64 front = 0;
                         uint32_t equal = 0;
                         for (uint32_t j = 0; j < members; j++) {
-                            if (keys[j] > key) before += weights[j];
+                            if (keys[j] > key) front += weights[j];
                             if (keys[j] == key) equal++;
                         }
-                        if (before < goal && goal <= before + equal * weights[i]) {  // all of that key agree
+                        if (front < goal && goal <= front + equal * weights[i]) {  // all of that key agree
                             s.pick_key = key;
                             s.pick_same = equal;
-                            s.pick_above = before;
+                            s.pick_above = front;
                         }
                     }
                     sync_block();
@@ -439,22 +604,24 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
                     // Many members: halve the range of their keys.  All above `hi` have the weight `above`,
                     // below the goal; with those from `lo` on it is reached.
                     uint32_t lo = 0xffffffffu, hi = 0;
-                    each([&](float x) {
-                        if (member(x)) lo = min(lo, key_of(x)), hi = max(hi, key_of(x));
+                    each([&](float v) {
+                        v = seen(v);
+                        if (member(v)) lo = min(lo, key_of(v)), hi = max(hi, key_of(v));
                     });
                     auto least = [](u64 a, u64 b) { return a < b ? a : b; };
-                    auto most = [](u64 a, u64 b) { return a > b ? a : b; };
+                    auto largest = [](u64 a, u64 b) { return a > b ? a : b; };
                     lo = (uint32_t)reduce(lo, 0xffffffffu, least);
-                    hi = (uint32_t)reduce(hi, 0, most);
+                    hi = (uint32_t)reduce(hi, 0, largest);
                     while (lo < hi) {
                         const uint32_t mid = lo + (hi - lo + 1) / 2;
                         u64 part = 0;
                         uint32_t under = 0, over = 0xffffffffu;  // the nearest keys on either side of mid
-                        each([&](float x) {
-                            const uint32_t key = key_of(x);
-                            if (key < lo || key > hi || !member(x)) return;
+                        each([&](float v) {
+                            v = seen(v);
+                            const uint32_t key = key_of(v);
+                            if (key < lo || key > hi || !member(v)) return;
                             if (key >= mid) {
-                                part += by_weight ? weight_of(exp_of(x, top, l.inv_t)) : 1;
+                                part += by_weight ? weight_of(exp_of(v, top, l.inv_t)) : 1;
                                 over = min(over, key);
                             } else {
                                 under = max(under, key);
@@ -465,12 +632,12 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
                             lo = (uint32_t)reduce(over, 0xffffffffu, least);
                         } else {
                             above += part;
-                            hi = (uint32_t)reduce(under, 0, most);
+                            hi = (uint32_t)reduce(under, 0, largest);
                         }
                     }
                     cut = lo;
                     u64 equal = 0;
-                    each([&](float x) { equal += key_of(x) == cut; });
+                    each([&](float v) { equal += key_of(seen(v)) == cut; });
                     same = (uint32_t)sum(equal);
                 }
                 const u64 each_w = by_weight ? weight_of(exp_of(score_of(cut), top, l.inv_t)) : 1;
@@ -482,18 +649,18 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
         u64 ties_before = 0;
         if (some) {
             u64 equal = 0;
-            each([&](float x) { equal += key_of(x) == cut; });
+            each([&](float v) { equal += key_of(seen(v)) == cut; });
             sum(equal, &ties_before);
         }
-        // The kept weight of each lane's step, in order: f(place, weights, their sum).
+        // The kept weight of each step, in order: f(place, weights, their sum).
         auto walk = [&](auto&& f) {
-            uint32_t seen = (uint32_t)ties_before;
-            each_step([&](const Pack<T, VEC>& p, uint32_t place) {
+            uint32_t passed = (uint32_t)ties_before;
+            each_step([&](const Pack<float, 4>& p, uint32_t place) {
                 uint32_t rank = 0;
                 if (some) {
                     uint32_t mine = 0;
 #pragma unroll
-                    for (int i = 0; i < VEC; i++) mine += key_of(to_f32(p.v[i])) == cut;
+                    for (int i = 0; i < 4; i++) mine += key_of(seen(p.v[i])) == cut;
                     rank = mine;
 #pragma unroll
                     for (int d = 1; d < 32; d *= 2) {
@@ -501,17 +668,17 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
                         if (lane >= d) rank += y;
                     }
                     const uint32_t all = __shfl_sync(0xffffffffu, rank, 31);
-                    rank += seen - mine;
-                    seen += all;
+                    rank += passed - mine;
+                    passed += all;
                 }
-                u64 w[VEC], sum = 0;
+                u64 w[4], sum = 0;
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    const float x = to_f32(p.v[i]);
-                    const uint32_t key = key_of(x);
+                for (int i = 0; i < 4; i++) {
+                    const float v = seen(p.v[i]);
+                    const uint32_t key = key_of(v);
                     w[i] = 0;
                     if (key > cut || (key == cut && (!some || rank < ties))) {
-                        const float e = exp_of(x, top, l.inv_t);
+                        const float e = exp_of(v, top, l.inv_t);
                         if (!(e < l.min_p)) w[i] = weight_of(e);
                     }
                     rank += key == cut;
@@ -539,7 +706,7 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
                 const u64 all = __shfl_sync(0xffffffffu, upto, 31);
                 u64 low = run + upto - sum;
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
+                for (int i = 0; i < 4; i++) {
                     if (place >= low && place < low + w[i]) {
                         out_classes[r] = (int32_t)(at + i - shift);
                         if (out_probs) out_probs[r] = share_of(w[i], total);
@@ -554,16 +721,18 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> struct RowDraw {
 
 constexpr int kRowsPerBlock = 4;  // of one warp each
 
-template <class T, int VEC, int NV, int WARPS, int CTAS>
+template <class T, bool HELD, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS == 1 ? 32 * kRowsPerBlock : 32 * WARPS)
-    k_sample_row(const T* __restrict__ scores, uint64_t n, uint32_t classes, uint64_t stride,
+    k_sample_row(const T* __restrict__ scores, uint64_t n, uint32_t classes, uint32_t steps, uint64_t stride,
                  const float* __restrict__ u, fbgpu_sample_params params, int32_t* __restrict__ out_classes,
                  float* __restrict__ out_probs) {
+    using Sh = RowShared<WARPS, CTAS>;
+    extern __shared__ __align__(16) unsigned char memory[];
     constexpr int kRows = WARPS == 1 ? kRowsPerBlock : 1;
-    __shared__ RowShared<WARPS, CTAS> shared[kRows];
-    RowDraw<T, VEC, NV, WARPS, CTAS> d(shared[WARPS == 1 ? threadIdx.x / 32 : 0]);
-    const uint64_t start = (uint64_t)(blockIdx.x / CTAS) * kRows + (WARPS == 1 ? threadIdx.x / 32 : 0);
-    for (uint64_t r = start; r < n; r += (uint64_t)(gridDim.x / CTAS) * kRows) {
+    const int mine = WARPS == 1 ? threadIdx.x / 32 : 0;
+    RowDraw<T, HELD, WARPS, CTAS> d(reinterpret_cast<Sh*>(memory)[mine],
+                                    reinterpret_cast<float*>(memory + kRows * sizeof(Sh)) + mine * steps * 128, steps);
+    for (uint64_t r = (uint64_t)(blockIdx.x / CTAS) * kRows + mine; r < n; r += (uint64_t)(gridDim.x / CTAS) * kRows) {
         d.open(scores + r * stride, classes);
         d.draw(r, params, u, out_classes, out_probs);
     }
@@ -587,11 +756,23 @@ template <class T, int KP> void launch_thread(const SampleArgs& a) {
                                                          a.u, a.params, a.out_classes, a.out_probs);
 }
 
-template <class T, int VEC, int NV, int WARPS, int CTAS> void launch_row(const SampleArgs& a) {
+// Steps of a warp for rows of `classes` classes, wherever they begin.
+template <class T> uint32_t steps_of(uint32_t classes, uint32_t warps) {
+    return ceil_div(classes + 16 / sizeof(T) - 1, warps * 128);
+}
+
+template <class T, bool HELD, int WARPS, int CTAS> void launch_row(const SampleArgs& a) {
+    using Sh = RowShared<WARPS, CTAS>;
     constexpr int kRows = WARPS == 1 ? kRowsPerBlock : 1;
+    const uint32_t steps = steps_of<T>(a.classes, WARPS * CTAS);
+    const size_t bytes = kRows * (sizeof(Sh) + (HELD ? (size_t)WARPS * steps * 128 * 4 : 0));
+    const auto kernel = k_sample_row<T, HELD, WARPS, CTAS>;
+    if (bytes > 48 << 10)
+        FB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((uint32_t)std::min<uint64_t>(1u << 18, (a.n + kRows - 1) / kRows) * CTAS);
     cfg.blockDim = dim3(32 * WARPS * kRows);
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = a.stream;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeClusterDimension;
@@ -599,24 +780,21 @@ template <class T, int VEC, int NV, int WARPS, int CTAS> void launch_row(const S
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = CTAS > 1 ? 1 : 0;
-    FB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sample_row<T, VEC, NV, WARPS, CTAS>, static_cast<const T*>(a.scores), a.n,
-                                     a.classes, a.stride, a.u, a.params, a.out_classes, a.out_probs));
+    FB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(a.scores), a.n, a.classes, steps, a.stride,
+                                     a.u, a.params, a.out_classes, a.out_probs));
 }
 
 template <class T> void launch_sample(const SampleArgs& a) {
-    constexpr int V = 16 / sizeof(T);  // elements of a vector
     count_launch();
-    const uint32_t k = a.classes, held = k + V - 1;  // places with the largest shift
+    const uint32_t k = a.classes;
     if (k <= 4) launch_thread<T, 4>(a);
     else if (k <= 8) launch_thread<T, 8>(a);
     else if (k <= 16) launch_thread<T, 16>(a);
-    else if (k <= 64) launch_row<T, 1, 2, 1, 1>(a);
-    else if (k <= 256) launch_row<T, 1, 8, 1, 1>(a);
-    else if (k <= 1024) launch_row<T, 1, 32, 1, 1>(a);
-    else if (held <= 8192) launch_row<T, V, 32 / V, 8, 1>(a);
-    else if (held <= 20480) launch_row<T, V, 40 / V, 16, 1>(a);
-    else if (held <= 163840) launch_row<T, V, 40 / V, 16, 8>(a);
-    else launch_row<T, V, 0, 16, 8>(a);
+    else if (k <= 1024) launch_row<T, true, 1, 1>(a);
+    else if (k <= 8192) launch_row<T, true, 8, 1>(a);
+    else if (k <= 32768 && a.n >= 64) launch_row<T, true, 16, 1>(a);
+    else if (k <= 262144) launch_row<T, true, 16, 8>(a);  // 32768 scores of a block: 128 KB
+    else launch_row<T, false, 16, 8>(a);
 }
 
 }  // namespace

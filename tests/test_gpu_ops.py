@@ -455,3 +455,32 @@ def test_launches_are_counted():
     before = _lib.load().fbgpu_launch_count()
     ops().embed(randn((5, 4), 1), tokens_of(3, 2, 5, 1))
     assert _lib.load().fbgpu_launch_count() == before + 1
+
+
+@pytest.mark.parametrize("K", [1024, 1025, 8192, 8193, 32768, 32769, 262144, 262145, 300001, 1 << 20])
+def test_sample_at_the_edges_of_the_variants(K):
+    """Sizes at which another kernel takes over, with many and few rows and a
+    row that starts off a 16-byte boundary."""
+    base = randn((2 * K + 3,), K, "bfloat16")
+    x = base[3:3 + 2 * K].view(2, K)
+    u = torch.rand(2, generator=gen(K), device="cuda")
+    for limits in ((1.0, 0, 1.0, 0.0), (0.7, 40, 0.9, 0.0), (1.0, 0, 0.5, 0.01), (1.0, K // 2, 0.95, 0.0), (1.0, 1000, 1.0, 0.0)):
+        c, p = check_draw(x, u, *limits)
+        if K <= 32769:
+            c64, p64 = ops().sample(x[[0, 1] * 40], u.repeat(40), temperature=limits[0], top_k=limits[1],
+                                    top_p=limits[2], min_p=limits[3])
+            assert torch.equal(c64, c.repeat(40)) and torch.equal(p64, p.repeat(40))
+
+
+@pytest.mark.parametrize("K", [700, 3000, 40000])
+def test_sample_temperatures_at_the_ends_of_f32(K):
+    x = randn((4, K), K)
+    u = torch.rand(4, generator=gen(1), device="cuda")
+    for t in (1e-45, 1e-38, 1e-20, 1e20, 3e38):
+        c, p = ops().sample(x, u, temperature=t, top_k=500, top_p=0.9)
+        if t < 1:
+            assert torch.equal(c, x.argmax(1).int()) and (p == 1).all()
+        else:  # every class weighs the same: 450 of the 500 largest are left, drawn by class
+            kept = x.argsort(dim=1, descending=True, stable=True)[:, :450].sort(1).values
+            want = kept.gather(1, (u.double() * 450).long()[:, None])[:, 0]
+            assert torch.equal(c.long(), want) and torch.allclose(p, torch.full_like(p, 1 / 450), rtol=2.0 ** -23)
