@@ -27,21 +27,26 @@ from . import _lib
 __all__ = ["embed", "embed_grad", "dropout", "sample"]
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # FBGPU_F32, FBGPU_F16, FBGPU_BF16
+_F32 = {torch.float32: 0}
 _TOKENS = {torch.int32: 0, torch.int64: 1}                        # FBGPU_I32, FBGPU_I64
+
+
+_lib_ = _lib.load()
+_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _type(name: str, t: Any, dims: int | None, types: dict) -> int:
     """The type code of a CUDA tensor, with its dimensions checked."""
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be on a CUDA device, it is on {t.device}")
-    if dims is not None and t.dim() != dims:
-        raise ValueError(f"{name} must have {dims} dimension(s), got shape {tuple(t.shape)}")
-    code = types.get(t.dtype)
-    if code is None:
+    if isinstance(t, torch.Tensor):
+        code = types.get(t.dtype)
+        if code is not None and t.is_cuda and (dims is None or t.dim() == dims):
+            return code
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be on a CUDA device, it is on {t.device}")
+        if dims is not None and t.dim() != dims:
+            raise ValueError(f"{name} must have {dims} dimension(s), got shape {tuple(t.shape)}")
         raise ValueError(f"{name} must be one of {', '.join(str(k) for k in types)}, got {t.dtype}")
-    return code
+    raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
 
 
 def _rows(name: str, t: torch.Tensor) -> int:
@@ -52,43 +57,39 @@ def _rows(name: str, t: torch.Tensor) -> int:
     return row
 
 
-def _same_device(t: torch.Tensor, **others: Any) -> None:
-    device = t.get_device()
-    for name, o in others.items():
-        if o is not None and o.get_device() != device:
-            raise ValueError(f"{name} is on cuda:{o.get_device()}, the other tensors are on cuda:{device}")
+def _same_device(name: str, t: torch.Tensor, device: int) -> None:
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors are on cuda:{device}")
 
 
 def _out(out: Any, shape: tuple, like: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
     if not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != like.dtype:
         raise ValueError(f"out must be a {like.dtype} tensor of shape {shape}")
-    _same_device(like, out=out)
+    _same_device("out", out, like.get_device())
     return out
 
 
-def _call(t: torch.Tensor, fn: str, *args: Any) -> None:
-    """Calls the entry point on t's device, with that device's current stream as the last argument."""
-    device = t.get_device()
-    f = getattr(_lib.load(), fn)
-    if device == torch.cuda.current_device():
-        status = f(*args, torch.cuda.current_stream(device).cuda_stream)
+def _call(device: int, f: Any, *args: Any) -> None:
+    """Calls the entry point on the device, with its current stream as the last argument."""
+    if device == _device():
+        status = f(*args, _stream(device))
     else:
         with torch.cuda.device(device):
-            status = f(*args, torch.cuda.current_stream(device).cuda_stream)
+            status = f(*args, _stream(device))
     if status:
-        message = (_lib.load().fbgpu_last_error(None) or b"").decode()
+        message = (_lib_.fbgpu_last_error(None) or b"").decode()
         raise (ValueError if status == 1 else RuntimeError)(message)
 
 
 def _token_shape(tokens: torch.Tensor) -> tuple:
     """(token code, rows, tokens per row, row stride, column stride)"""
     code = _type("tokens", tokens, None, _TOKENS)
-    if tokens.dim() == 1:
+    dims = tokens.dim()
+    if dims == 1:
         return code, tokens.shape[0], 1, tokens.stride(0), 1
-    if tokens.dim() == 2:
-        return code, tokens.shape[0], tokens.shape[1], tokens.stride(0), tokens.stride(1)
+    if dims == 2:
+        n, k = tokens.shape
+        return (code, n, k, *tokens.stride())
     raise ValueError(f"tokens must have 1 or 2 dimensions, got shape {tuple(tokens.shape)}")
 
 
@@ -109,11 +110,12 @@ def embed(table: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0,
     Returns n x dim in the table's type."""
     code = _type("table", table, 2, _TYPES)
     tcode, n, k, trow, tcol = _token_shape(tokens)
-    _same_device(table, tokens=tokens)
+    device = table.get_device()
+    _same_device("tokens", tokens, device)
     vocab, dim = table.shape
     _count(dim, k)
-    out = _out(out, (n, dim), table)
-    _call(table, "fbgpu_embed", table.data_ptr(), code, vocab, dim, _rows("table", table), tokens.data_ptr(), tcode, n,
+    out = table.new_empty((n, dim)) if out is None else _out(out, (n, dim), table)
+    _call(device, _lib_.fbgpu_embed, table.data_ptr(), code, vocab, dim, _rows("table", table), tokens.data_ptr(), tcode, n,
           k, trow, tcol, scale, out.data_ptr(), _rows("out", out))
     return out
 
@@ -129,7 +131,8 @@ def embed_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale: f
     atomic adds are used.  n * k and vocab are at most 2**31 - 2."""
     code = _type("grad", grad, 2, _TYPES)
     tcode, n, k, trow, tcol = _token_shape(tokens)
-    _same_device(grad, tokens=tokens)
+    device = grad.get_device()
+    _same_device("tokens", tokens, device)
     vocab = int(vocab)
     if vocab < 0:
         raise ValueError(f"vocab must not be negative, got {vocab}")
@@ -137,10 +140,10 @@ def embed_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale: f
         raise ValueError(f"grad has {grad.shape[0]} rows, tokens has {n}")
     dim = grad.shape[1]
     _count(dim, k)
-    out = _out(out, (vocab, dim), grad)
-    size = _lib.load().fbgpu_embed_grad_workspace(n, k, vocab, dim)
-    space = torch.empty(size, dtype=torch.uint8, device=grad.device)
-    _call(grad, "fbgpu_embed_grad", grad.data_ptr(), code, n, k, dim, _rows("grad", grad), tokens.data_ptr(), tcode,
+    out = grad.new_empty((vocab, dim)) if out is None else _out(out, (vocab, dim), grad)
+    size = _lib_.fbgpu_embed_grad_workspace(n, k, vocab, dim)
+    space = grad.new_empty(size, dtype=torch.uint8)
+    _call(device, _lib_.fbgpu_embed_grad, grad.data_ptr(), code, n, k, dim, _rows("grad", grad), tokens.data_ptr(), tcode,
           trow, tcol, vocab, scale, out.data_ptr(), _rows("out", out), space.data_ptr(), size)
     return out
 
@@ -157,7 +160,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, *,
     contiguous rows.  ``out=x`` works in place."""
     code = _type("x", x, None, _TYPES)
     p = float(p)
-    out = _out(out, tuple(x.shape), x)
+    out = x.new_empty(x.shape) if out is None else _out(out, tuple(x.shape), x)
     if x.is_contiguous() and out.is_contiguous():
         n, dim = 1, x.numel()
         xs = os = dim
@@ -167,7 +170,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, *,
     else:
         raise ValueError(f"x and out must be contiguous, or 2-D with contiguous rows; x has shape {tuple(x.shape)} "
                          f"and strides {x.stride()}")
-    _call(x, "fbgpu_dropout", x.data_ptr(), code, n, dim, xs, p, seed & 0xFFFFFFFFFFFFFFFF,
+    _call(x.get_device(), _lib_.fbgpu_dropout, x.data_ptr(), code, n, dim, xs, p, seed & 0xFFFFFFFFFFFFFFFF,
           offset & 0xFFFFFFFFFFFFFFFF, out.data_ptr(), os)
     return out
 
@@ -178,8 +181,15 @@ def _limit(name: str, value: Any, scores: torch.Tensor, dtype: torch.dtype) -> t
         return value, None
     if value.dtype != dtype or value.shape != scores.shape[:1] or not value.is_contiguous():
         raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {scores.shape[0]} values")
-    _same_device(scores, **{name: value})
+    _same_device(name, value, scores.get_device())
     return 0, value.data_ptr()
+
+
+def _result(name: str, t: Any, u: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != u.shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {u.shape[0]} values")
+    _same_device(name, t, u.get_device())
+    return t
 
 
 def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: Any = 1.0, top_k: Any = 0, top_p: Any = 1.0,
@@ -202,10 +212,11 @@ def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: Any = 1.0, top
     sums; classes below that are never drawn."""
     code = _type("scores", scores, 2, _TYPES)
     n, k = scores.shape
-    _type("u", u, 1, {torch.float32: 0})
+    _type("u", u, 1, _F32)
     if u.shape[0] != n or not u.is_contiguous():
         raise ValueError(f"u must be contiguous with {n} values, got shape {tuple(u.shape)}")
-    _same_device(scores, u=u)
+    device = scores.get_device()
+    _same_device("u", u, device)
     t, ts = _limit("temperature", temperature, scores, torch.float32)
     tk, tks = _limit("top_k", top_k, scores, torch.int32)
     tp, tps = _limit("top_p", top_p, scores, torch.float32)
@@ -214,15 +225,9 @@ def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: Any = 1.0, top
         raise ValueError(f"top_k must be a whole number in 0..2**31 - 1, got {tk}")
     if k > 1 << 20:
         raise ValueError(f"classes must be in 2..1048576, got {k}")
-    if classes is None:
-        classes = torch.empty(n, dtype=torch.int32, device=scores.device)
-    if probs is None:
-        probs = torch.empty(n, dtype=torch.float32, device=scores.device)
-    for name, t_, dtype in (("classes", classes, torch.int32), ("probs", probs, torch.float32)):
-        if t_.dtype != dtype or t_.shape != u.shape or not t_.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values")
-        _same_device(scores, **{name: t_})
+    classes = u.new_empty(n, dtype=torch.int32) if classes is None else _result("classes", classes, u, torch.int32)
+    probs = u.new_empty(n) if probs is None else _result("probs", probs, u, torch.float32)
     params = _lib.FbgpuSampleParams(t, int(tk), tp, mp, ts, tks, tps, mps)
-    _call(scores, "fbgpu_sample", scores.data_ptr(), code, n, k, _rows("scores", scores), u.data_ptr(),
+    _call(device, _lib_.fbgpu_sample, scores.data_ptr(), code, n, k, _rows("scores", scores), u.data_ptr(),
           C.byref(params), classes.data_ptr(), probs.data_ptr())
     return classes, probs
