@@ -156,10 +156,197 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
     }
 }
 
-// ------------------------------------------- a warp, block or cluster per row
+// -------------------------------------------------- a few lanes of a warp per row
+// L lanes (1 to 32) hold a row in registers, lane l the classes [E * l, E * l + E).
+// A limit's threshold is found by halving the range of scores it lies in: each
+// round sums what is at or above the middle, and the range's new end is the
+// nearest score on its side of the middle, so that about log2(classes) rounds
+// find it.  Fewer lanes a row mean fewer rounds for the warp's rows together; a
+// lane's 32 scores and weights are what its registers take.
+template <class T, int L, int E>
+__global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scores, uint64_t n, uint32_t classes,
+                                                      uint64_t stride, const float* __restrict__ u,
+                                                      fbgpu_sample_params params, int32_t* __restrict__ out_classes,
+                                                      float* __restrict__ out_probs) {
+    constexpr int kRows = 128 / L;
+    constexpr uint32_t kAll = 0xffffffffu;
+    __shared__ float staged[128 * (E + 1)];  // a lane's scores one word apart from the next lane's banks
+    const int lane = threadIdx.x & (L - 1);
+    float* const own = staged + threadIdx.x * (E + 1);
+    auto add_lanes = [](u64 v) {
+#pragma unroll
+        for (int d = L / 2; d; d /= 2) v += __shfl_xor_sync(kAll, v, d);
+        return v;
+    };
+    auto largest = [](float v) {
+#pragma unroll
+        for (int d = L / 2; d; d /= 2) v = fmaxf(v, __shfl_xor_sync(kAll, v, d));
+        return v;
+    };
+    // the rows of a warp stay together: one past the end works on the last row and writes nothing
+    for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < n; r0 += (uint64_t)gridDim.x * kRows) {
+        const uint64_t at = r0 + threadIdx.x / L, r = min(at, n - 1);
+        __syncwarp();
+        if (L == 1) {
+            const T* row = scores + r * stride;
+            for (int c = 0; c < E; c++) own[c] = c < classes ? score(to_f32(row[c])) : -INFINITY;
+        } else {
+            const T* row = scores + r * stride;
+#pragma unroll 4
+            for (int c = lane; c < L * E; c += L) {
+                float* to = own - lane * (E + 1) + c / E * (E + 1) + c % E;
+                *to = c < classes ? score(to_f32(row[c])) : -INFINITY;
+            }
+        }
+        __syncwarp();
+        const Limits l = limits_of(params, r, classes);
+        float x[E], top = -INFINITY, bottom = INFINITY;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            x[i] = own[i];
+            top = fmaxf(top, x[i]);
+        }
+        top = largest(top);
+        if (top == INFINITY) {  // only the infinite ones weigh
+#pragma unroll
+            for (int i = 0; i < E; i++) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+            top = 0.0f;
+        }
+        const bool empty = top == -INFINITY;
+        u64 w[E];
+        uint32_t count = 0, kept = 0;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const float e = exp_of(x[i], top, l.inv_t);
+            w[i] = x[i] > -INFINITY ? weight_of(e) : 0;
+            if (!(e < l.min_p)) kept |= 1u << i;
+            if (x[i] > -INFINITY) count++, bottom = fminf(bottom, x[i]);
+        }
+        bottom = -largest(-bottom);
+        count = (uint32_t)add_lanes(count);
+        // kept: above `cut`, or equal to it and one of the first `ties` of the `same` of that score
+        float cut = -INFINITY;
+        uint32_t ties = kAll, same = 0;
+        if (l.greedy) cut = top, ties = 1, same = kAll;
+#pragma unroll 1
+        for (int by_weight = 0; by_weight < 2; by_weight++) {
+            bool find = !l.greedy && !empty && (by_weight ? l.use_p : l.top_k < count);
+            if (!__any_sync(kAll, find)) continue;
+            const float w_cut = exp_of(cut, top, l.inv_t);
+            u64 goal = l.top_k;
+            if (by_weight) {
+                u64 total = 0;
+#pragma unroll
+                for (int i = 0; i < E; i++) total += x[i] > cut ? w[i] : 0;
+                total = add_lanes(total);
+                if (ties < kAll) total += min(ties, same) * weight_of(w_cut);
+                goal = goal_of(l.top_p, total);
+                find = find && goal <= total;
+            }
+            float lo = by_weight ? fmaxf(bottom, cut) : bottom, hi = top;
+            u64 above = 0;
+            while (__any_sync(kAll, find && lo < hi)) {
+                float mid = fminf(__fadd_rn(__fmul_rn(lo, 0.5f), __fmul_rn(hi, 0.5f)), hi);
+                if (!(mid > lo)) mid = hi;
+                u64 part = 0;
+                if (by_weight) {
+#pragma unroll
+                    for (int i = 0; i < E; i++) part += x[i] >= mid && x[i] <= hi ? w[i] : 0;
+                } else {
+                    uint32_t some = 0;
+#pragma unroll
+                    for (int i = 0; i < E; i++) some += x[i] >= mid && x[i] <= hi;
+                    part = some;
+                }
+                part = add_lanes(part);
+                const bool reached = above + part >= goal;
+                // the nearest score at or above the middle, or below it
+                float near = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < E; i++) {
+                    const float v = reached ? -x[i] : x[i], end = reached ? -mid : mid;
+                    if (reached ? v <= end : v < end) near = fmaxf(near, v);
+                }
+                near = largest(near);
+                if (find && lo < hi) {
+                    if (reached) lo = -near;
+                    else above += part, hi = near;
+                }
+            }
+            uint32_t equal = 0;
+#pragma unroll
+            for (int i = 0; i < E; i++) equal += x[i] == lo;
+            equal = (uint32_t)add_lanes(equal);
+            if (find) {
+                cut = lo;
+                same = equal;
+                goal -= above;
+                if (by_weight) {
+                    const u64 one = weight_of(exp_of(cut, top, l.inv_t));
+                    ties = same == 1 ? 1 : (uint32_t)((goal + one - 1) / one);
+                } else {
+                    ties = (uint32_t)goal;
+                }
+            }
+        }
+        if (__any_sync(kAll, ties < same)) {  // the lane's first class of the score `cut`, counted over the row
+            uint32_t mine = 0;
+#pragma unroll
+            for (int i = 0; i < E; i++) mine += x[i] == cut;
+            uint32_t rank = mine;
+#pragma unroll
+            for (int d = 1; d < L; d *= 2) {
+                const uint32_t y = __shfl_up_sync(kAll, rank, d, L);
+                if (lane >= d) rank += y;
+            }
+            rank -= mine;
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                if (x[i] == cut) {
+                    if (rank >= ties) kept &= ~(1u << i);
+                    rank++;
+                }
+            }
+        }
+        u64 mine = 0;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            if (!(x[i] >= cut) || !(kept >> i & 1)) w[i] = 0;
+            mine += w[i];
+        }
+        u64 upto = mine;
+#pragma unroll
+        for (int d = 1; d < L; d *= 2) {
+            const u64 y = __shfl_up_sync(kAll, upto, d, L);
+            if (lane >= d) upto += y;
+        }
+        const u64 total = __shfl_sync(kAll, upto, L - 1, L);
+        if (at >= n) continue;
+        if (empty) {
+            if (lane == 0) {
+                out_classes[r] = -1;
+                if (out_probs) out_probs[r] = 0.0f;
+            }
+            continue;
+        }
+        const u64 place = place_of(u[r], total);
+        u64 run = upto - mine, won = 0;
+        if (place < run || place >= upto) continue;  // another lane's
+        int drawn = 0;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            if (place >= run && place < run + w[i]) drawn = i, won = w[i];
+            run += w[i];
+        }
+        out_classes[r] = lane * E + drawn;
+        if (out_probs) out_probs[r] = share_of(won, total);
+    }
+}
+
+// ------------------------------------------------- a block or cluster per row
 // WARPS warps of CTAS blocks (one cluster) hold a row.  Its scores are brought
-// into shared memory as f32 once (HELD; a row too long for that is read again
-// for every step) and every later step is a short loop over them: held in
+// into shared memory as f32 once (HELD; other rows are read again for every
+// step, from the L2) and every later step is a short loop over them: held in
 // registers, the unrolled steps ran out of the instruction cache.  Places are
 // counted from the 16-byte boundary at or before the row's first class, so that
 // the loads are aligned vectors; the places before that class, and after the
@@ -168,9 +355,7 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
 constexpr int kSort = 1024;  // the most classes that are sorted
 
 template <int WARPS, int CTAS> struct alignas(16) RowShared {
-    static constexpr int kBins = WARPS == 1 ? 256 : 1024;
-    static constexpr int kList = WARPS == 1 ? 64 : 128;
-    static constexpr int kSorted = WARPS == 1 ? 1 : kSort;
+    static constexpr int kBins = 1024, kList = 128;
     uint32_t low[kBins], high[kBins];     // a bin's count, or its weight as two words
     u64 part[2][WARPS];                   // warps' partial sums; two sets, used in turn
     uint32_t found[3];                    // members of the chosen bin; of the list to sort
@@ -179,7 +364,9 @@ template <int WARPS, int CTAS> struct alignas(16) RowShared {
     u64 scan[WARPS];
     u64 before, pick_above;
     uint32_t bin, pick_key, pick_same;
-    u64 sorted[kSorted], sorted_weight[kSorted];
+    u64 sorted[kSort], sorted_weight[kSort];
+    u64 chunk[WARPS][8];                  // a warp's kept weight in eighths of its part
+    uint32_t chunk_ties[WARPS][8];        // and the row's classes of the threshold's score before each
 };
 
 template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
@@ -197,19 +384,15 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
 
     __device__ __forceinline__ RowDraw(Sh& sh, float* held, uint32_t steps_) : s(sh), x(held), steps(steps_) {
         lane = threadIdx.x & 31;
-        warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
-        tid = WARPS == 1 ? lane : threadIdx.x;
+        warp = threadIdx.x >> 5;
+        tid = threadIdx.x;
         cta = CTAS == 1 ? 0 : (int)cooperative_groups::this_cluster().block_rank();
         block_first = cta * WARPS * steps * kStep;
         warp_first = block_first + warp * steps * kStep;
     }
 
-    __device__ __forceinline__ void sync_block() {
-        if (WARPS == 1) __syncwarp();
-        else __syncthreads();
-    }
     __device__ __forceinline__ void sync_row() {
-        if (CTAS == 1) sync_block();
+        if (CTAS == 1) __syncthreads();
         else cooperative_groups::this_cluster().sync();
     }
     // Another block's shared memory.
@@ -228,7 +411,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         shift = (uint32_t)(((uintptr_t)row % 16) / sizeof(T));
         if (!HELD) return;
         most = -INFINITY;
-        sync_block();  // the row before is no longer read
+        __syncthreads();  // the row before is no longer read
         const uint32_t vectors = WARPS * steps * kStep / V;
         for (uint32_t v0 = tid; v0 < vectors; v0 += kAhead * kThreads) {
             union {
@@ -260,23 +443,39 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                     *reinterpret_cast<float4*>(x + v * V + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
             }
         }
-        sync_block();
+        __syncthreads();
     }
-    // f(scores, place of the first) for each of the lane's steps, in order
-    template <class F> __device__ __forceinline__ void each_step(F&& f) {
+    // f(scores, place of the first) for the lane's steps [from, to), in order
+    template <class F> __device__ __forceinline__ void steps_of_warp(uint32_t from, uint32_t to, F&& f) {
+        constexpr int kAhead = HELD ? 1 : 4;
 #pragma unroll 1
-        for (uint32_t i = 0; i < steps; i++) {
-            const uint32_t place = warp_first + i * kStep + lane * 4;
-            Pack<float, 4> p;
+        for (uint32_t i = from; i < to; i += kAhead) {
+            Pack<float, 4> p[kAhead];
             if (HELD) {
-                p = *reinterpret_cast<const Pack<float, 4>*>(x + (place - block_first));
+                p[0] = *reinterpret_cast<const Pack<float, 4>*>(x + (warp_first - block_first) + i * kStep + lane * 4);
             } else {
+                Pack<T, 4> q[kAhead];
+                bool whole[kAhead];
 #pragma unroll
-                for (int k = 0; k < 4; k++) p.v[k] = one(place + k);
+                for (int k = 0; k < kAhead; k++) {
+                    const uint32_t place = warp_first + (i + k) * kStep + lane * 4;
+                    whole[k] = place >= shift && place + 4 <= shift + classes;
+                    q[k] = *(whole[k] ? reinterpret_cast<const Pack<T, 4>*>(row + (place - shift))
+                                      : reinterpret_cast<const Pack<T, 4>*>(&g_zero));
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; k++) {
+                    const uint32_t place = warp_first + (i + k) * kStep + lane * 4;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) p[k].v[j] = whole[k] ? score(to_f32(q[k].v[j])) : one(place + j);
+                }
             }
-            f(p, place);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++)
+                if (i + k < to) f(p[k], warp_first + (i + k) * kStep + lane * 4);
         }
     }
+    template <class F> __device__ __forceinline__ void each_step(F&& f) { steps_of_warp(0, steps, f); }
     // f(score) for each of the lane's places
     template <class F> __device__ __forceinline__ void each(F&& f) {
         each_step([&](const Pack<float, 4>& p, uint32_t) {
@@ -291,7 +490,6 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
 #pragma unroll
         for (int d = 16; d; d /= 2) v = op(v, (u64)__shfl_xor_sync(0xffffffffu, v, d));
         if (before) *before = zero;
-        if (WARPS == 1) return v;
         if (lane == 0) s.part[parity][warp] = v;
         sync_row();
         u64 all = zero, front = zero;
@@ -322,21 +520,17 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
             const u64 y = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= d) upto += y;
         }
-        total = __shfl_sync(0xffffffffu, upto, 31);
-        if (WARPS > 1) {
-            sync_block();
-            if (lane == 31) s.scan[warp] = upto;
-            sync_block();
-            u64 all = lane < WARPS ? s.scan[lane] : 0, front = lane < warp ? all : 0;
+        __syncthreads();
+        if (lane == 31) s.scan[warp] = upto;
+        __syncthreads();
+        u64 all = lane < WARPS ? s.scan[lane] : 0, front = lane < warp ? all : 0;
 #pragma unroll
-            for (int d = 16; d; d /= 2) {
-                all += __shfl_xor_sync(0xffffffffu, all, d);
-                front += __shfl_xor_sync(0xffffffffu, front, d);
-            }
-            total = all;
-            upto += front;
+        for (int d = 16; d; d /= 2) {
+            all += __shfl_xor_sync(0xffffffffu, all, d);
+            front += __shfl_xor_sync(0xffffffffu, front, d);
         }
-        return upto - mine;
+        total = all;
+        return upto - mine + front;
     }
 
     __device__ __forceinline__ uint32_t bin_of(float v, float top, float per) {
@@ -345,7 +539,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     __device__ __forceinline__ void clear_bins(int set) {
         for (int i = tid; i < kBins; i += kThreads) s.low[i] = s.high[i] = 0;
         if (tid == 0) s.found[set] = 0, s.bin = kBins;
-        sync_block();
+        __syncthreads();
     }
     // After the bins are filled: the bin in which the running sum reaches the goal that goal_for(total) names
     // (kBins: none), and the sum before it.  Every block of a cluster does the same work.
@@ -371,7 +565,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
             }
             run += v[i];
         }
-        sync_block();
+        __syncthreads();
         before = s.before;
         return s.bin;
     }
@@ -385,7 +579,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                     const u64 u = a[lo], v = a[hi];
                     if ((u < v) == ((lo & k) == 0)) a[lo] = v, a[hi] = u;
                 }
-                sync_block();
+                __syncthreads();
             }
         }
     }
@@ -397,7 +591,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         uint32_t count = 32;
         while (count < members) count *= 2;
         for (uint32_t i = members + tid; i < count; i += kThreads) s.sorted[i] = 0;
-        sync_block();
+        __syncthreads();
         sort(s.sorted, count);
         u64 item[kPer], w[kPer], mine = 0, total;
         float e[kPer];
@@ -428,7 +622,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         block_before(mine, total);
         uint32_t kept = 32;
         while (kept < members && kept < l.top_k) kept *= 2;
-        sync_block();
+        __syncthreads();
         sort(s.sorted, kept);
         mine = 0;
 #pragma unroll
@@ -473,7 +667,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         auto seen = [&](float v) { return certain ? (v == INFINITY ? FLT_MAX : -INFINITY) : v; };
         // Weights vanish 27.73 T below the maximum: bins over that span, falling, the last for the rest.
         const float per = __fmul_rn(kBins / 27.75f, l.inv_t);
-        if (WARPS > 1 && !l.greedy && l.top_k < classes && l.top_k <= kSort) {
+        if (!l.greedy && l.top_k < classes && l.top_k <= kSort) {
             // At least top_k classes are at or above the top_k-th largest of the threads' maxima: those are sorted.
             clear_bins(2);
             if (HELD && l.top_k * 4 <= kThreads * CTAS) {
@@ -580,7 +774,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                         }
                         keys = s.all_key;
                         weights = s.all_weight;
-                        sync_block();
+                        __syncthreads();
                     }
                     for (uint32_t i = tid; i < members; i += kThreads) {
                         const uint32_t key = keys[i];
@@ -596,7 +790,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                             s.pick_above = front;
                         }
                     }
-                    sync_block();
+                    __syncthreads();
                     cut = s.pick_key;
                     same = s.pick_same;
                     above = s.pick_above;
@@ -652,10 +846,9 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
             each([&](float v) { equal += key_of(seen(v)) == cut; });
             sum(equal, &ties_before);
         }
-        // The kept weight of each step, in order: f(place, weights, their sum).
-        auto walk = [&](auto&& f) {
-            uint32_t passed = (uint32_t)ties_before;
-            each_step([&](const Pack<float, 4>& p, uint32_t place) {
+        // The kept weight of steps [from, to), in order: f(place, weights, their sum).
+        auto walk = [&](uint32_t from, uint32_t to, uint32_t& passed, auto&& f) {
+            steps_of_warp(from, to, [&](const Pack<float, 4>& p, uint32_t place) {
                 uint32_t rank = 0;
                 if (some) {
                     uint32_t mine = 0;
@@ -687,16 +880,30 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 f(place, w, sum);
             });
         };
+        // the warp's weight by eighths of its part, so that only one eighth is walked again
+        const uint32_t eighth = (steps + 7) / 8;
+        uint32_t passed = (uint32_t)ties_before;
         u64 mine = 0, before = 0;
-        walk([&](uint32_t, u64*, u64 w) { mine += w; });
-        u64 part = mine;
+#pragma unroll 1
+        for (uint32_t e = 0; e < 8; e++) {
+            const uint32_t ties_here = passed;
+            u64 part = 0;
+            if (e * eighth < steps) {
+                walk(e * eighth, min(steps, (e + 1) * eighth), passed, [&](uint32_t, u64*, u64 w) { part += w; });
+                mine += part;
 #pragma unroll
-        for (int d = 16; d; d /= 2) part += __shfl_xor_sync(0xffffffffu, part, d);
+                for (int d = 16; d; d /= 2) part += __shfl_xor_sync(0xffffffffu, part, d);
+            }
+            if (lane == 0) s.chunk[warp][e] = part, s.chunk_ties[warp][e] = ties_here;
+        }
         const u64 total = sum(mine, &before);
         const u64 place = place_of(u[r], total);
-        if (place >= before && place < before + part) {  // this warp holds the class
+        uint32_t e = 0;
+        while (e < 8 && place >= before && place >= before + s.chunk[warp][e]) before += s.chunk[warp][e++];
+        if (place >= before && e < 8) {  // this warp holds the class
             u64 run = before;
-            walk([&](uint32_t at, u64* w, u64 sum) {
+            passed = s.chunk_ties[warp][e];
+            walk(e * eighth, min(steps, (e + 1) * eighth), passed, [&](uint32_t at, u64* w, u64 sum) {
                 u64 upto = sum;
 #pragma unroll
                 for (int d = 1; d < 32; d *= 2) {
@@ -719,20 +926,15 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     }
 };
 
-constexpr int kRowsPerBlock = 4;  // of one warp each
-
-template <class T, bool HELD, int WARPS, int CTAS>
-__global__ void __launch_bounds__(WARPS == 1 ? 32 * kRowsPerBlock : 32 * WARPS)
+template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS>
+__global__ void __launch_bounds__(32 * WARPS, BLOCKS)
     k_sample_row(const T* __restrict__ scores, uint64_t n, uint32_t classes, uint32_t steps, uint64_t stride,
                  const float* __restrict__ u, fbgpu_sample_params params, int32_t* __restrict__ out_classes,
                  float* __restrict__ out_probs) {
     using Sh = RowShared<WARPS, CTAS>;
     extern __shared__ __align__(16) unsigned char memory[];
-    constexpr int kRows = WARPS == 1 ? kRowsPerBlock : 1;
-    const int mine = WARPS == 1 ? threadIdx.x / 32 : 0;
-    RowDraw<T, HELD, WARPS, CTAS> d(reinterpret_cast<Sh*>(memory)[mine],
-                                    reinterpret_cast<float*>(memory + kRows * sizeof(Sh)) + mine * steps * 128, steps);
-    for (uint64_t r = (uint64_t)(blockIdx.x / CTAS) * kRows + mine; r < n; r += (uint64_t)(gridDim.x / CTAS) * kRows) {
+    RowDraw<T, HELD, WARPS, CTAS> d(*reinterpret_cast<Sh*>(memory), reinterpret_cast<float*>(memory + sizeof(Sh)), steps);
+    for (uint64_t r = blockIdx.x / CTAS; r < n; r += gridDim.x / CTAS) {
         d.open(scores + r * stride, classes);
         d.draw(r, params, u, out_classes, out_probs);
     }
@@ -756,22 +958,27 @@ template <class T, int KP> void launch_thread(const SampleArgs& a) {
                                                          a.u, a.params, a.out_classes, a.out_probs);
 }
 
+template <class T, int L, int E> void launch_lanes(const SampleArgs& a) {
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>(1u << 20, (a.n + 128 / L - 1) / (128 / L));
+    k_sample_lanes<T, L, E><<<blocks, 128, 0, a.stream>>>(static_cast<const T*>(a.scores), a.n, a.classes, a.stride,
+                                                          a.u, a.params, a.out_classes, a.out_probs);
+}
+
 // Steps of a warp for rows of `classes` classes, wherever they begin.
 template <class T> uint32_t steps_of(uint32_t classes, uint32_t warps) {
     return ceil_div(classes + 16 / sizeof(T) - 1, warps * 128);
 }
 
-template <class T, bool HELD, int WARPS, int CTAS> void launch_row(const SampleArgs& a) {
+template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(const SampleArgs& a) {
     using Sh = RowShared<WARPS, CTAS>;
-    constexpr int kRows = WARPS == 1 ? kRowsPerBlock : 1;
     const uint32_t steps = steps_of<T>(a.classes, WARPS * CTAS);
-    const size_t bytes = kRows * (sizeof(Sh) + (HELD ? (size_t)WARPS * steps * 128 * 4 : 0));
-    const auto kernel = k_sample_row<T, HELD, WARPS, CTAS>;
+    const size_t bytes = sizeof(Sh) + (HELD ? (size_t)WARPS * steps * 128 * 4 : 0);
+    const auto kernel = k_sample_row<T, HELD, WARPS, CTAS, BLOCKS>;
     if (bytes > 48 << 10)
         FB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((uint32_t)std::min<uint64_t>(1u << 18, (a.n + kRows - 1) / kRows) * CTAS);
-    cfg.blockDim = dim3(32 * WARPS * kRows);
+    cfg.gridDim = dim3((uint32_t)std::min<uint64_t>(1u << 18, a.n) * CTAS);
+    cfg.blockDim = dim3(32 * WARPS);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = a.stream;
     cudaLaunchAttribute at{};
@@ -790,11 +997,15 @@ template <class T> void launch_sample(const SampleArgs& a) {
     if (k <= 4) launch_thread<T, 4>(a);
     else if (k <= 8) launch_thread<T, 8>(a);
     else if (k <= 16) launch_thread<T, 16>(a);
-    else if (k <= 1024) launch_row<T, true, 1, 1>(a);
-    else if (k <= 8192) launch_row<T, true, 8, 1>(a);
-    else if (k <= 32768 && a.n >= 64) launch_row<T, true, 16, 1>(a);
-    else if (k <= 262144) launch_row<T, true, 16, 8>(a);  // 32768 scores of a block: 128 KB
-    else launch_row<T, false, 16, 8>(a);
+    else if (k <= 32) launch_lanes<T, 1, 32>(a);
+    else if (k <= 64) launch_lanes<T, 2, 32>(a);
+    else if (k <= 128) launch_lanes<T, 4, 32>(a);
+    else if (k <= 256) launch_lanes<T, 8, 32>(a);
+    else if (k <= 2048) launch_row<T, true, 4, 1, 8>(a);
+    else if (k <= 8192) launch_row<T, true, 8, 1, 3>(a);
+    else if (a.n >= 64) launch_row<T, false, 16, 1, 2>(a);
+    else if (k <= 262144) launch_row<T, true, 16, 8, 1>(a);  // 32768 scores of a block: 128 KB
+    else launch_row<T, false, 16, 8, 1>(a);
 }
 
 }  // namespace
