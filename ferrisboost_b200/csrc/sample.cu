@@ -355,18 +355,21 @@ __global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scor
 constexpr int kSort = 1024;  // the most classes that are sorted
 
 template <int WARPS, int CTAS> struct alignas(16) RowShared {
-    static constexpr int kBins = 1024, kList = 128;
+    static constexpr int kBins = 1024, kPick = 128;
     uint32_t low[kBins], high[kBins];     // a bin's count, or its weight as two words
     u64 part[2][WARPS];                   // warps' partial sums; two sets, used in turn
     uint32_t found[3];                    // members of the chosen bin; of the list to sort
-    uint32_t key[2][kList], all_key[kList];
-    u64 weight[2][kList], all_weight[kList];
+    uint32_t all_key[kPick];
+    u64 all_weight[kPick];
     u64 scan[WARPS];
     u64 before, pick_above;
-    uint32_t bin, pick_key, pick_same;
-    u64 sorted[kSort], sorted_weight[kSort];
+    uint32_t bin, pick_key, pick_same, tie_place;
+    union {
+        uint32_t key[2][kSort];           // members of the chosen bin
+        u64 sorted[kSort];
+    };
+    u64 sorted_weight[kSort];
     u64 chunk[WARPS][8];                  // a warp's kept weight in eighths of its part
-    uint32_t chunk_ties[WARPS][8];        // and the row's classes of the threshold's score before each
 };
 
 template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
@@ -396,12 +399,15 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         else cooperative_groups::this_cluster().sync();
     }
     // Another block's shared memory.
-    template <class V> __device__ __forceinline__ const V* at(const V* p, int c) {
+    template <class V> __device__ __forceinline__ V* at(V* p, int c) {
         if (CTAS == 1) return p;
         return cooperative_groups::this_cluster().map_shared_rank(p, c);
     }
     __device__ __forceinline__ float one(uint32_t place) {
-        return place >= shift && place < shift + classes ? score(to_f32(row[place - shift])) : -INFINITY;
+        return place >= shift && place < shift + classes ? to_f32(row[place - shift]) : -INFINITY;
+    }
+    __device__ __forceinline__ bool inside(uint32_t place, uint32_t count) {
+        return place >= shift && place + count <= shift + classes;
     }
 
     __device__ __forceinline__ void open(const T* row_, uint32_t classes_) {
@@ -418,12 +424,10 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 uint4 u;
                 T v[V];
             } p[kAhead];
-            bool whole[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
                 const uint32_t place = block_first + (v0 + k * kThreads) * V;
-                whole[k] = place >= shift && place + V <= shift + classes;
-                p[k].u = *(whole[k] ? reinterpret_cast<const uint4*>(row + (place - shift)) : &g_zero);
+                p[k].u = *(inside(place, V) ? reinterpret_cast<const uint4*>(row + (place - shift)) : &g_zero);
             }
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
@@ -431,8 +435,8 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 if (v >= vectors) break;
                 float f[V];
 #pragma unroll
-                for (int i = 0; i < V; i++) f[i] = score(to_f32(p[k].v[i]));
-                if (!whole[k]) {
+                for (int i = 0; i < V; i++) f[i] = to_f32(p[k].v[i]);
+                if (!inside(place, V)) {
 #pragma unroll
                     for (int i = 0; i < V; i++) f[i] = one(place + i);
                 }
@@ -445,34 +449,40 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         }
         __syncthreads();
     }
-    // f(scores, place of the first) for the lane's steps [from, to), in order
+    // f(four scores, place of the first) for the lane's steps [from, to), in order.  A score may be NaN.
     template <class F> __device__ __forceinline__ void steps_of_warp(uint32_t from, uint32_t to, F&& f) {
-        constexpr int kAhead = HELD ? 1 : 4;
+        if (HELD) {
+            const float* mine = x + (warp_first - block_first) + lane * 4;
+#pragma unroll 2
+            for (uint32_t i = from; i < to; i++)
+                f(*reinterpret_cast<const Pack<float, 4>*>(mine + i * kStep), warp_first + i * kStep + lane * 4);
+            return;
+        }
+        constexpr int kAhead = 4;
 #pragma unroll 1
         for (uint32_t i = from; i < to; i += kAhead) {
-            Pack<float, 4> p[kAhead];
-            if (HELD) {
-                p[0] = *reinterpret_cast<const Pack<float, 4>*>(x + (warp_first - block_first) + i * kStep + lane * 4);
-            } else {
+            const uint32_t place = warp_first + i * kStep + lane * 4;
+            if (i + kAhead <= to && inside(warp_first + i * kStep, kAhead * kStep)) {
                 Pack<T, 4> q[kAhead];
-                bool whole[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; k++)
+                    q[k] = *reinterpret_cast<const Pack<T, 4>*>(row + (place - shift) + k * kStep);
 #pragma unroll
                 for (int k = 0; k < kAhead; k++) {
-                    const uint32_t place = warp_first + (i + k) * kStep + lane * 4;
-                    whole[k] = place >= shift && place + 4 <= shift + classes;
-                    q[k] = *(whole[k] ? reinterpret_cast<const Pack<T, 4>*>(row + (place - shift))
-                                      : reinterpret_cast<const Pack<T, 4>*>(&g_zero));
+                    Pack<float, 4> p;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) p.v[j] = to_f32(q[k].v[j]);
+                    f(p, place + k * kStep);
                 }
+            } else {
+#pragma unroll 1
+                for (uint32_t k = 0; k < kAhead && i + k < to; k++) {
+                    Pack<float, 4> p;
 #pragma unroll
-                for (int k = 0; k < kAhead; k++) {
-                    const uint32_t place = warp_first + (i + k) * kStep + lane * 4;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) p[k].v[j] = whole[k] ? score(to_f32(q[k].v[j])) : one(place + j);
+                    for (int j = 0; j < 4; j++) p.v[j] = one(place + k * kStep + j);
+                    f(p, place + k * kStep);
                 }
             }
-#pragma unroll
-            for (int k = 0; k < kAhead; k++)
-                if (i + k < to) f(p[k], warp_first + (i + k) * kStep + lane * 4);
         }
     }
     template <class F> __device__ __forceinline__ void each_step(F&& f) { steps_of_warp(0, steps, f); }
@@ -533,9 +543,9 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         return upto - mine + front;
     }
 
-    __device__ __forceinline__ uint32_t bin_of(float v, float top, float per) {
-        return min((uint32_t)(kBins - 1), __float2uint_rz(__fmul_rn(__fsub_rn(top, v), per)));
-    }
+    // How far a score lies below the maximum, in bins.
+    __device__ __forceinline__ float depth(float v, float top, float per) { return __fmul_rn(__fsub_rn(top, v), per); }
+    __device__ __forceinline__ uint32_t bin_of(float d) { return min((uint32_t)(kBins - 1), __float2uint_rz(d)); }
     __device__ __forceinline__ void clear_bins(int set) {
         for (int i = tid; i < kBins; i += kThreads) s.low[i] = s.high[i] = 0;
         if (tid == 0) s.found[set] = 0, s.bin = kBins;
@@ -647,13 +657,11 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     __device__ __forceinline__ void draw(uint64_t r, const fbgpu_sample_params& params, const float* u,
                                          int32_t* out_classes, float* out_probs) {
         const Limits l = limits_of(params, r, classes);
-        float top = -INFINITY;
-        if (HELD) top = most;
-        else each([&](float v) { top = fmaxf(top, v); });
-        {
-            const uint32_t k = (uint32_t)reduce(key_of(top), 0, [](u64 a, u64 b) { return a > b ? a : b; });
-            top = score_of(k);
+        if (!HELD) {
+            most = -INFINITY;
+            each([&](float v) { most = fmaxf(most, v); });
         }
+        const float top = score_of((uint32_t)reduce(key_of(score(most)), 0, [](u64 a, u64 b) { return a > b ? a : b; }));
         if (top == -INFINITY) {
             if (tid == 0 && cta == 0) {
                 out_classes[r] = -1;
@@ -661,31 +669,28 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
             }
             return;
         }
-        const bool certain = top == INFINITY;  // only the infinite ones weigh
-        if (certain) top = FLT_MAX;
-        // Scores as they count: +infinity as FLT_MAX, and then everything else as -infinity.
-        auto seen = [&](float v) { return certain ? (v == INFINITY ? FLT_MAX : -INFINITY) : v; };
         // Weights vanish 27.73 T below the maximum: bins over that span, falling, the last for the rest.
-        const float per = __fmul_rn(kBins / 27.75f, l.inv_t);
-        if (!l.greedy && l.top_k < classes && l.top_k <= kSort) {
+        const float per = fminf(__fmul_rn(kBins / 27.75f, l.inv_t), FLT_MAX);
+        if (!l.greedy && top < INFINITY && l.top_k < classes && l.top_k <= kSort) {
             // At least top_k classes are at or above the top_k-th largest of the threads' maxima: those are sorted.
             clear_bins(2);
-            if (HELD && l.top_k * 4 <= kThreads * CTAS) {
-                if (seen(most) > -INFINITY) atomicAdd(&s.low[bin_of(seen(most), top, per)], 1u);
+            if (l.top_k * 4 <= kThreads * CTAS) {
+                if (most > -INFINITY) atomicAdd(&s.low[bin_of(depth(most, top, per))], 1u);
             } else {
                 each([&](float v) {
-                    if (seen(v) > -INFINITY) atomicAdd(&s.low[bin_of(seen(v), top, per)], 1u);
+                    if (v > -INFINITY) atomicAdd(&s.low[bin_of(depth(v, top, per))], 1u);
                 });
             }
             u64 before, goal;
             const uint32_t bin = find_bin(before, goal, [&](u64) { return (u64)l.top_k; });
+            const float end = bin >= kBins - 1 ? INFINITY : bin + 1.0f;
             each_step([&](const Pack<float, 4>& p, uint32_t place) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float v = seen(p.v[i]);
-                    if (v > -INFINITY && bin_of(v, top, per) <= bin) {
+                    const float d = depth(p.v[i], top, per);
+                    if (d < end || (end == INFINITY && p.v[i] > -INFINITY)) {
                         const uint32_t q = atomicAdd(&s.found[2], 1u);
-                        if (q < kSort) s.sorted[q] = (u64)key_of(v) << 32 | ~(place + i - shift);
+                        if (q < kSort) s.sorted[q] = (u64)key_of(score(p.v[i])) << 32 | ~(place + i - shift);
                     }
                 }
             });
@@ -705,12 +710,20 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 return;
             }
         }
-        // kept: key > cut, or key == cut and one of the first `ties` of the `same` classes of that key
-        uint32_t cut = 0, ties = 0xffffffffu, same = 0;
+        // kept: above `cut`, or equal to it and one of the first `ties` of the `same` classes of that score
+        float cut = -INFINITY;
+        uint32_t ties = 0xffffffffu, same = 0;
         if (l.greedy) {
-            cut = key_of(top);
+            cut = top;
             ties = 1;
             same = 0xffffffffu;
+        } else if (top == INFINITY) {  // the infinite ones alone, of one weight
+            u64 count = 0;
+            each([&](float v) { count += v == INFINITY; });
+            cut = top;
+            same = (uint32_t)sum(count);
+            ties = min(l.top_k, same);
+            if (l.use_p) ties = (uint32_t)((goal_of(l.top_p, (u64)ties << 40) + (1ull << 40) - 1) >> 40);
         } else {
             // first by count for top_k, then by weight for top_p
 #pragma unroll 1
@@ -718,9 +731,8 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 if (by_weight ? !l.use_p : l.top_k >= classes) continue;
                 clear_bins(by_weight);
                 each([&](float v) {
-                    v = seen(v);
-                    if (v == -INFINITY || key_of(v) < cut) return;
-                    const uint32_t b = bin_of(v, top, per);
+                    if (!(v >= cut && v > -INFINITY)) return;
+                    const uint32_t b = bin_of(depth(v, top, per));
                     if (by_weight) {
                         const u64 w = weight_of(exp_of(v, top, l.inv_t));
                         if (w == 0) return;
@@ -734,7 +746,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 u64 before, goal;
                 const uint32_t bin = find_bin(before, goal, [&](u64 total) -> u64 {
                     if (!by_weight) return l.top_k;
-                    if (ties < same) total -= (same - ties) * weight_of(exp_of(score_of(cut), top, l.inv_t));
+                    if (ties < same) total -= (same - ties) * weight_of(exp_of(cut, top, l.inv_t));
                     return goal_of(l.top_p, total);
                 });
                 if (bin == kBins) {  // the whole row stays below the goal
@@ -743,65 +755,75 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 }
                 goal -= before;
                 // the chosen bin's members
+                const float start = bin, end = bin == kBins - 1 ? INFINITY : bin + 1.0f;
                 auto member = [&](float v) {
-                    return v > -INFINITY && key_of(v) >= cut && bin_of(v, top, per) == bin;
+                    const float d = depth(v, top, per);
+                    return v >= cut && v > -INFINITY && d >= start && (d < end || end == INFINITY);
                 };
+                uint32_t* const list = s.key[by_weight];
                 each([&](float v) {
-                    v = seen(v);
                     if (!member(v)) return;
                     const uint32_t q = atomicAdd(&s.found[by_weight], 1u);
-                    if (q < Sh::kList) {
-                        s.key[by_weight][q] = key_of(v);
-                        s.weight[by_weight][q] = by_weight ? weight_of(exp_of(v, top, l.inv_t)) : 1;
-                    }
+                    if (q < kSort) list[q] = key_of(score(v));
                 });
                 sync_row();
                 uint32_t members = 0;
-                for (int c = 0; c < CTAS; c++) members += *at(&s.found[by_weight], c);
+                bool listed = true;
+                for (int c = 0; c < CTAS; c++) {
+                    const uint32_t m = *at(&s.found[by_weight], c);
+                    members += m;
+                    listed = listed && m <= kSort;
+                }
+                auto weight = [&](uint32_t key) -> u64 {
+                    return by_weight ? weight_of(exp_of(score_of(key), top, l.inv_t)) : 1;
+                };
                 u64 above = 0;
-                if (members <= Sh::kList) {
-                    const uint32_t* keys = s.key[by_weight];
-                    const u64* weights = s.weight[by_weight];
-                    if (CTAS > 1) {
-                        uint32_t base = 0;
-                        for (int c = 0; c < CTAS; c++) {
-                            const uint32_t m = *at(&s.found[by_weight], c);
-                            for (uint32_t i = tid; i < m; i += kThreads) {
-                                s.all_key[base + i] = at(s.key[by_weight], c)[i];
-                                s.all_weight[base + i] = at(s.weight[by_weight], c)[i];
-                            }
-                            base += m;
+                uint32_t key = 0;
+                if (members <= Sh::kPick) {  // few: each is compared with all
+                    uint32_t base = 0;
+                    for (int c = 0; c < CTAS; c++) {
+                        const uint32_t m = *at(&s.found[by_weight], c);
+                        for (uint32_t i = tid; i < m; i += kThreads) {
+                            const uint32_t k = at(list, c)[i];
+                            s.all_key[base + i] = k;
+                            s.all_weight[base + i] = weight(k);
                         }
-                        keys = s.all_key;
-                        weights = s.all_weight;
-                        __syncthreads();
+                        base += m;
                     }
+                    __syncthreads();
                     for (uint32_t i = tid; i < members; i += kThreads) {
-                        const uint32_t key = keys[i];
+                        const uint32_t k = s.all_key[i];
                         u64 front = 0;
                         uint32_t equal = 0;
                         for (uint32_t j = 0; j < members; j++) {
-                            if (keys[j] > key) front += weights[j];
-                            if (keys[j] == key) equal++;
+                            if (s.all_key[j] > k) front += s.all_weight[j];
+                            if (s.all_key[j] == k) equal++;
                         }
-                        if (front < goal && goal <= front + equal * weights[i]) {  // all of that key agree
-                            s.pick_key = key;
+                        if (front < goal && goal <= front + equal * s.all_weight[i]) {  // all of that key agree
+                            s.pick_key = k;
                             s.pick_same = equal;
                             s.pick_above = front;
                         }
                     }
                     __syncthreads();
-                    cut = s.pick_key;
+                    key = s.pick_key;
                     same = s.pick_same;
                     above = s.pick_above;
                 } else {
-                    // Many members: halve the range of their keys.  All above `hi` have the weight `above`,
-                    // below the goal; with those from `lo` on it is reached.
+                    // Many: halve the range of their keys.  All above `hi` have the weight `above`, below the
+                    // goal; with those from `lo` on it is reached.  The ends are keys that occur, so that a bin
+                    // of one score is done at once.
+                    auto each_member = [&](auto&& f) {
+                        if (listed) {
+                            for (uint32_t i = tid; i < s.found[by_weight]; i += kThreads) f(list[i]);
+                        } else {
+                            each([&](float v) {
+                                if (member(v)) f(key_of(score(v)));
+                            });
+                        }
+                    };
                     uint32_t lo = 0xffffffffu, hi = 0;
-                    each([&](float v) {
-                        v = seen(v);
-                        if (member(v)) lo = min(lo, key_of(v)), hi = max(hi, key_of(v));
-                    });
+                    each_member([&](uint32_t k) { lo = min(lo, k), hi = max(hi, k); });
                     auto least = [](u64 a, u64 b) { return a < b ? a : b; };
                     auto largest = [](u64 a, u64 b) { return a > b ? a : b; };
                     lo = (uint32_t)reduce(lo, 0xffffffffu, least);
@@ -810,15 +832,13 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                         const uint32_t mid = lo + (hi - lo + 1) / 2;
                         u64 part = 0;
                         uint32_t under = 0, over = 0xffffffffu;  // the nearest keys on either side of mid
-                        each([&](float v) {
-                            v = seen(v);
-                            const uint32_t key = key_of(v);
-                            if (key < lo || key > hi || !member(v)) return;
-                            if (key >= mid) {
-                                part += by_weight ? weight_of(exp_of(v, top, l.inv_t)) : 1;
-                                over = min(over, key);
+                        each_member([&](uint32_t k) {
+                            if (k < lo || k > hi) return;
+                            if (k >= mid) {
+                                part += weight(k);
+                                over = min(over, k);
                             } else {
-                                under = max(under, key);
+                                under = max(under, k);
                             }
                         });
                         part = sum(part);
@@ -829,81 +849,90 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                             hi = (uint32_t)reduce(under, 0, largest);
                         }
                     }
-                    cut = lo;
+                    key = lo;
                     u64 equal = 0;
-                    each([&](float v) { equal += key_of(seen(v)) == cut; });
+                    each_member([&](uint32_t k) { equal += k == key; });
                     same = (uint32_t)sum(equal);
                 }
-                const u64 each_w = by_weight ? weight_of(exp_of(score_of(cut), top, l.inv_t)) : 1;
+                cut = score_of(key);
+                const u64 each_w = weight(key);
                 ties = (uint32_t)((goal - above + each_w - 1) / each_w);
             }
         }
-        // How many of the key `cut` come before this warp's part, where not all of them are kept.
-        const bool some = ties < same;
-        u64 ties_before = 0;
-        if (some) {
-            u64 equal = 0;
-            each([&](float v) { equal += key_of(seen(v)) == cut; });
-            sum(equal, &ties_before);
-        }
-        // The kept weight of steps [from, to), in order: f(place, weights, their sum).
-        auto walk = [&](uint32_t from, uint32_t to, uint32_t& passed, auto&& f) {
-            steps_of_warp(from, to, [&](const Pack<float, 4>& p, uint32_t place) {
-                uint32_t rank = 0;
-                if (some) {
-                    uint32_t mine = 0;
+        // Where not all classes of the score `cut` are kept: the last place that is.
+        uint32_t tie_place = 0xffffffffu;
+        if (ties < same) {
+            u64 equal = 0, front;
+            each([&](float v) { equal += v == cut; });
+            const uint32_t mine = __reduce_add_sync(0xffffffffu, (uint32_t)equal);
+            sum(equal, &front);
+            if (front < ties && ties <= front + mine) {  // in this warp's part
+                uint32_t passed = (uint32_t)front;
+                steps_of_warp(0, steps, [&](const Pack<float, 4>& p, uint32_t place) {
+                    uint32_t here = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) mine += key_of(seen(p.v[i])) == cut;
-                    rank = mine;
+                    for (int i = 0; i < 4; i++) here += p.v[i] == cut;
+                    const uint32_t all = __reduce_add_sync(0xffffffffu, here);
+                    if (passed < ties && ties <= passed + all) {
+                        uint32_t upto = here;
 #pragma unroll
-                    for (int d = 1; d < 32; d *= 2) {
-                        const uint32_t y = __shfl_up_sync(0xffffffffu, rank, d);
-                        if (lane >= d) rank += y;
+                        for (int d = 1; d < 32; d *= 2) {
+                            const uint32_t y = __shfl_up_sync(0xffffffffu, upto, d);
+                            if (lane >= d) upto += y;
+                        }
+                        uint32_t rank = passed + upto - here;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            if (p.v[i] == cut && ++rank == ties)
+                                for (int c = 0; c < CTAS; c++) *at(&s.tie_place, c) = place + i;
+                        }
                     }
-                    const uint32_t all = __shfl_sync(0xffffffffu, rank, 31);
-                    rank += passed - mine;
                     passed += all;
-                }
-                u64 w[4], sum = 0;
+                });
+            }
+            sync_row();
+            tie_place = s.tie_place;
+        }
+        // The kept weights of a step.
+        auto weigh = [&](const Pack<float, 4>& p, uint32_t place, u64* w) -> u64 {
+            u64 sum = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float v = seen(p.v[i]);
-                    const uint32_t key = key_of(v);
-                    w[i] = 0;
-                    if (key > cut || (key == cut && (!some || rank < ties))) {
-                        const float e = exp_of(v, top, l.inv_t);
-                        if (!(e < l.min_p)) w[i] = weight_of(e);
-                    }
-                    rank += key == cut;
-                    sum += w[i];
+            for (int i = 0; i < 4; i++) {
+                const float v = p.v[i];
+                w[i] = 0;
+                if (v > cut || (v == cut && place + i <= tie_place)) {
+                    const float e = v == top ? 1.0f : exp_of(v, top, l.inv_t);
+                    if (!(e < l.min_p)) w[i] = weight_of(e);
                 }
-                f(place, w, sum);
-            });
+                sum += w[i];
+            }
+            return sum;
         };
         // the warp's weight by eighths of its part, so that only one eighth is walked again
         const uint32_t eighth = (steps + 7) / 8;
-        uint32_t passed = (uint32_t)ties_before;
         u64 mine = 0, before = 0;
 #pragma unroll 1
         for (uint32_t e = 0; e < 8; e++) {
-            const uint32_t ties_here = passed;
             u64 part = 0;
-            if (e * eighth < steps) {
-                walk(e * eighth, min(steps, (e + 1) * eighth), passed, [&](uint32_t, u64*, u64 w) { part += w; });
-                mine += part;
+            steps_of_warp(min(steps, e * eighth), min(steps, (e + 1) * eighth), [&](const Pack<float, 4>& p, uint32_t place) {
+                u64 w[4];
+                part += weigh(p, place, w);
+            });
+            mine += part;
 #pragma unroll
-                for (int d = 16; d; d /= 2) part += __shfl_xor_sync(0xffffffffu, part, d);
-            }
-            if (lane == 0) s.chunk[warp][e] = part, s.chunk_ties[warp][e] = ties_here;
+            for (int d = 16; d; d /= 2) part += __shfl_xor_sync(0xffffffffu, part, d);
+            if (lane == 0) s.chunk[warp][e] = part;
         }
+        __syncwarp();
         const u64 total = sum(mine, &before);
         const u64 place = place_of(u[r], total);
         uint32_t e = 0;
         while (e < 8 && place >= before && place >= before + s.chunk[warp][e]) before += s.chunk[warp][e++];
         if (place >= before && e < 8) {  // this warp holds the class
             u64 run = before;
-            passed = s.chunk_ties[warp][e];
-            walk(e * eighth, min(steps, (e + 1) * eighth), passed, [&](uint32_t at, u64* w, u64 sum) {
+            steps_of_warp(min(steps, e * eighth), min(steps, (e + 1) * eighth), [&](const Pack<float, 4>& p, uint32_t at) {
+                u64 w[4];
+                const u64 sum = weigh(p, at, w);
                 u64 upto = sum;
 #pragma unroll
                 for (int d = 1; d < 32; d *= 2) {
