@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scor
             const T* row = scores + r * stride;
 #pragma unroll 4
             for (int c = lane; c < L * E; c += L) {
-                float* to = own - lane * (E + 1) + c / E * (E + 1) + c % E;
+                float* to = own + (c / E - lane) * (E + 1) + c % E;
                 *to = c < classes ? score(to_f32(row[c])) : -INFINITY;
             }
         }
@@ -244,33 +244,39 @@ __global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scor
                 find = find && goal <= total;
             }
             float lo = by_weight ? fmaxf(bottom, cut) : bottom, hi = top;
-            u64 above = 0;
+            u64 above = 0;  // what is above `hi`, below the goal
             while (__any_sync(kAll, find && lo < hi)) {
                 float mid = fminf(__fadd_rn(__fmul_rn(lo, 0.5f), __fmul_rn(hi, 0.5f)), hi);
                 if (!(mid > lo)) mid = hi;
+                // what is at or above the middle, and the nearest scores on either side of it
+                constexpr int kSums = 4;  // chains of additions
+                float over[2] = {INFINITY, INFINITY}, under[2] = {-INFINITY, -INFINITY};
                 u64 part = 0;
                 if (by_weight) {
+                    u64 sums[kSums] = {};
 #pragma unroll
-                    for (int i = 0; i < E; i++) part += x[i] >= mid && x[i] <= hi ? w[i] : 0;
+                    for (int i = 0; i < E; i++) {
+                        if (x[i] >= mid) sums[i % kSums] += w[i], over[i & 1] = fminf(over[i & 1], x[i]);
+                        else under[i & 1] = fmaxf(under[i & 1], x[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kSums; i++) part += sums[i];
                 } else {
-                    uint32_t some = 0;
+                    uint32_t sums[kSums] = {};
 #pragma unroll
-                    for (int i = 0; i < E; i++) some += x[i] >= mid && x[i] <= hi;
-                    part = some;
+                    for (int i = 0; i < E; i++) {
+                        if (x[i] >= mid) sums[i % kSums]++, over[i & 1] = fminf(over[i & 1], x[i]);
+                        else under[i & 1] = fmaxf(under[i & 1], x[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kSums; i++) part += sums[i];
                 }
                 part = add_lanes(part);
-                const bool reached = above + part >= goal;
-                // the nearest score at or above the middle, or below it
-                float near = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < E; i++) {
-                    const float v = reached ? -x[i] : x[i], end = reached ? -mid : mid;
-                    if (reached ? v <= end : v < end) near = fmaxf(near, v);
-                }
-                near = largest(near);
+                const bool reached = part >= goal;
+                const float near = largest(reached ? -fminf(over[0], over[1]) : fmaxf(under[0], under[1]));
                 if (find && lo < hi) {
                     if (reached) lo = -near;
-                    else above += part, hi = near;
+                    else above = part, hi = near;
                 }
             }
             uint32_t equal = 0;
@@ -351,11 +357,10 @@ __global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scor
 // counted from the 16-byte boundary at or before the row's first class, so that
 // the loads are aligned vectors; the places before that class, and after the
 // last, hold -infinity.  Block after block, and in it warp after warp, takes
-// a contiguous part of the places; a step is four of a lane.
-constexpr int kSort = 1024;  // the most classes that are sorted
-
+// a contiguous part of the places; a step is four of a lane.  Up to kSort classes
+// are sorted, and short rows take fewer bins.
 template <int WARPS, int CTAS> struct alignas(16) RowShared {
-    static constexpr int kBins = 1024, kPick = 128;
+    static constexpr int kBins = WARPS == 4 ? 256 : 1024, kSort = WARPS == 4 ? 512 : 1024, kPick = 128;
     uint32_t low[kBins], high[kBins];     // a bin's count, or its weight as two words
     u64 part[2][WARPS];                   // warps' partial sums; two sets, used in turn
     uint32_t found[3];                    // members of the chosen bin; of the list to sort
@@ -374,7 +379,7 @@ template <int WARPS, int CTAS> struct alignas(16) RowShared {
 
 template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     using Sh = RowShared<WARPS, CTAS>;
-    static constexpr int kBins = Sh::kBins, kThreads = WARPS * 32, kStep = 128;
+    static constexpr int kBins = Sh::kBins, kSort = Sh::kSort, kThreads = WARPS * 32, kStep = 128;
 
     Sh& s;
     float* x;             // HELD: the block's places
@@ -545,7 +550,10 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
 
     // How far a score lies below the maximum, in bins.
     __device__ __forceinline__ float depth(float v, float top, float per) { return __fmul_rn(__fsub_rn(top, v), per); }
-    __device__ __forceinline__ uint32_t bin_of(float d) { return min((uint32_t)(kBins - 1), __float2uint_rz(d)); }
+    // The nearest whole number by the addition of 2^23, whose low bits it becomes; monotone like the depth.
+    __device__ __forceinline__ uint32_t bin_of(float d) {
+        return __float_as_uint(__fadd_rn(fminf(d, kBins - 1.0f), 8388608.0f)) & (kBins - 1);
+    }
     __device__ __forceinline__ void clear_bins(int set) {
         for (int i = tid; i < kBins; i += kThreads) s.low[i] = s.high[i] = 0;
         if (tid == 0) s.found[set] = 0, s.bin = kBins;
@@ -683,12 +691,11 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
             }
             u64 before, goal;
             const uint32_t bin = find_bin(before, goal, [&](u64) { return (u64)l.top_k; });
-            const float end = bin >= kBins - 1 ? INFINITY : bin + 1.0f;
+            const float end = bin >= kBins - 1 ? INFINITY : bin + 0.5f;  // and what is rounded down from just there
             each_step([&](const Pack<float, 4>& p, uint32_t place) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float d = depth(p.v[i], top, per);
-                    if (d < end || (end == INFINITY && p.v[i] > -INFINITY)) {
+                    if (depth(p.v[i], top, per) <= end && p.v[i] > -INFINITY) {
                         const uint32_t q = atomicAdd(&s.found[2], 1u);
                         if (q < kSort) s.sorted[q] = (u64)key_of(score(p.v[i])) << 32 | ~(place + i - shift);
                     }
@@ -755,10 +762,8 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 }
                 goal -= before;
                 // the chosen bin's members
-                const float start = bin, end = bin == kBins - 1 ? INFINITY : bin + 1.0f;
                 auto member = [&](float v) {
-                    const float d = depth(v, top, per);
-                    return v >= cut && v > -INFINITY && d >= start && (d < end || end == INFINITY);
+                    return v >= cut && v > -INFINITY && bin_of(depth(v, top, per)) == bin;
                 };
                 uint32_t* const list = s.key[by_weight];
                 each([&](float v) {
@@ -919,8 +924,10 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 part += weigh(p, place, w);
             });
             mine += part;
+            if (e * eighth < steps) {
 #pragma unroll
-            for (int d = 16; d; d /= 2) part += __shfl_xor_sync(0xffffffffu, part, d);
+                for (int d = 16; d; d /= 2) part += __shfl_xor_sync(0xffffffffu, part, d);
+            }
             if (lane == 0) s.chunk[warp][e] = part;
         }
         __syncwarp();
@@ -1023,9 +1030,17 @@ template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(c
 template <class T> void launch_sample(const SampleArgs& a) {
     count_launch();
     const uint32_t k = a.classes;
-    if (k <= 4) launch_thread<T, 4>(a);
+    if (k <= 2) launch_thread<T, 2>(a);
+    else if (k <= 3) launch_thread<T, 3>(a);
+    else if (k <= 4) launch_thread<T, 4>(a);
+    else if (k <= 5) launch_thread<T, 5>(a);
+    else if (k <= 6) launch_thread<T, 6>(a);
+    else if (k <= 7) launch_thread<T, 7>(a);
     else if (k <= 8) launch_thread<T, 8>(a);
+    else if (k <= 10) launch_thread<T, 10>(a);
+    else if (k <= 12) launch_thread<T, 12>(a);
     else if (k <= 16) launch_thread<T, 16>(a);
+    else if (k <= 24) launch_lanes<T, 1, 24>(a);
     else if (k <= 32) launch_lanes<T, 1, 32>(a);
     else if (k <= 64) launch_lanes<T, 2, 32>(a);
     else if (k <= 128) launch_lanes<T, 4, 32>(a);
