@@ -129,7 +129,7 @@ struct BagArgs {
     float scale;
 };
 
-template <class T, class Tok, int V>
+template <class T, class Tok, int V, bool FLAT>  // FLAT: a row's tokens are next to one another
 __global__ void __launch_bounds__(kBagThreads, 4) k_embed(BagArgs a, const T* __restrict__ table, Tokens<Tok> tokens,
                                                           T* __restrict__ out) {
     using P = Pack<T, V>;
@@ -145,25 +145,41 @@ __global__ void __launch_bounds__(kBagThreads, 4) k_embed(BagArgs a, const T* __
         Sums<V> sum;
         sum.clear();
         if (r < a.n && c < a.dim) {
-            const Tok* tok = tokens.p + r * tokens.row;
-            const T* column = table + c;
+            const uint64_t col = FLAT ? 1 : tokens.col;
+            const Tok* tok = tokens.p + r * tokens.row + begin * col;
+            const char* column = reinterpret_cast<const char*>(table + c);
+            const uint64_t stride = a.table_stride * sizeof(T);
+            const U vocab = tokens.vocab;
+            auto row = [&](U t) {
+                return t < vocab ? reinterpret_cast<const P*>(column + t * stride) : reinterpret_cast<const P*>(&g_zero);
+            };
+            const uint32_t whole = (end - begin) / kBagAhead;
             U t[kBagAhead];
+            if (whole) {
 #pragma unroll
-            for (int k = 0; k < kBagAhead; k++)
-                t[k] = begin + k < end ? (U)tok[(begin + k) * tokens.col] : tokens.vocab;
-            for (uint32_t j = begin; j < end; j += kBagAhead) {
+                for (int k = 0; k < kBagAhead; k++) t[k] = (U)tok[k * col];
+            }
+            for (uint32_t j = 0; j < whole; j++) {
                 P e[kBagAhead];
 #pragma unroll
-                for (int k = 0; k < kBagAhead; k++)
-                    e[k] = *(t[k] < tokens.vocab ? reinterpret_cast<const P*>(column + t[k] * a.table_stride)
-                                                 : reinterpret_cast<const P*>(&g_zero));
+                for (int k = 0; k < kBagAhead; k++) e[k] = *row(t[k]);
+                tok += kBagAhead * col;
+                if (j + 1 < whole) {
 #pragma unroll
-                for (int k = 0; k < kBagAhead; k++) {
-                    const uint32_t next = j + kBagAhead + k;
-                    t[k] = next < end ? (U)tok[next * tokens.col] : tokens.vocab;
+                    for (int k = 0; k < kBagAhead; k++) t[k] = (U)tok[k * col];
                 }
 #pragma unroll
                 for (int k = 0; k < kBagAhead; k++) sum.add(e[k]);
+            }
+            const uint32_t rest = end - begin - whole * kBagAhead;
+            if (rest) {
+#pragma unroll
+                for (int k = 0; k < kBagAhead - 1; k++) t[k] = k < rest ? (U)tok[k * col] : vocab;
+                P e[kBagAhead];
+#pragma unroll
+                for (int k = 0; k < kBagAhead - 1; k++) e[k] = *row(t[k]);
+#pragma unroll
+                for (int k = 0; k < kBagAhead - 1; k++) sum.add(e[k]);
             }
         }
         if (a.parts_log) {
@@ -498,37 +514,46 @@ __global__ void __launch_bounds__(kRunThreads, 3) k_run_sums(RunSums a, const T*
     bool head = from_before;  // the current run is the one that came in
     Sums<V> acc;
     acc.clear();
-    for (uint32_t p = 0; p < a.chunk; p += kAhead) {
-        uint32_t key[kAhead], row[kAhead];
-        Pack<T, V> g[kAhead];
+    // every place of the chunk holds a token: nothing to check
+    const bool whole = begin + a.chunk <= a.count && a.items[begin + a.chunk - 1].x < a.vocab;
+    auto batches = [&](auto checked) {
+        constexpr bool kChecked = decltype(checked)::value;
+        for (uint32_t p = 0; p < a.chunk; p += kAhead) {
+            uint32_t key[kAhead], row[kAhead];
+            Pack<T, V> g[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; k += 2) {  // the list has room for the last pair
-            const uint64_t i = begin + p + k;
-            const uint4 two = i < a.count ? *reinterpret_cast<const uint4*>(a.items + i) : make_uint4(0, 0, 0, 0);
-            key[k] = i < a.count ? two.x : a.vocab;
-            row[k] = key[k] < a.vocab ? two.y : 0;
-            key[k + 1] = i + 1 < a.count ? two.z : a.vocab;
-            row[k + 1] = key[k + 1] < a.vocab ? two.w : 0;
-        }
-        // a missing token's place, and a lane past the last column, read something that is not used
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) g[k] = *reinterpret_cast<const Pack<T, V>*>(from + row[k] * a.grad_stride);
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            if (key[k] != cur) {
-                if (head) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc.v[i];
-                } else if (column) {
-                    write_row<T, V>(a, out, cur, c, acc);
+            for (int k = 0; k < kAhead; k += 2) {  // the list has room for the last pair
+                const uint64_t i = begin + p + k;
+                uint4 two = make_uint4(a.vocab, 0, a.vocab, 0);
+                if (!kChecked || i < a.count) two = *reinterpret_cast<const uint4*>(a.items + i);
+                key[k] = two.x, row[k] = two.y, key[k + 1] = two.z, row[k + 1] = two.w;
+                if (kChecked) {  // a place without a token reads row 0, which is not used
+                    if (i + 1 >= a.count) key[k + 1] = a.vocab;
+                    if (key[k] >= a.vocab) row[k] = 0;
+                    if (key[k + 1] >= a.vocab) row[k + 1] = 0;
                 }
-                head = false;
-                cur = key[k];
-                acc.clear();
             }
-            acc.add(g[k]);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) g[k] = *reinterpret_cast<const Pack<T, V>*>(from + row[k] * a.grad_stride);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                if (key[k] != cur) {
+                    if (head) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc.v[i];
+                    } else if (column) {
+                        write_row<T, V>(a, out, cur, c, acc);
+                    }
+                    head = false;
+                    cur = key[k];
+                    acc.clear();
+                }
+                acc.add(g[k]);
+            }
         }
-    }
+    };
+    if (whole) batches(std::false_type{});
+    else batches(std::true_type{});
     const bool to_after = cur < a.vocab && key_at(a, begin + a.chunk) == cur;
     if (head) {
 #pragma unroll
@@ -735,8 +760,12 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
                 with_type(type, [&](auto e) {
                     using T = decltype(e);
                     with_width<T>(v, [&](auto w) {
-                        k_embed<T, Tok, decltype(w)::value><<<grid, kBagThreads, 0, s>>>(
-                            a, static_cast<const T*>(table), tk, static_cast<T*>(out));
+                        if (token_col == 1)
+                            k_embed<T, Tok, decltype(w)::value, true><<<grid, kBagThreads, 0, s>>>(
+                                a, static_cast<const T*>(table), tk, static_cast<T*>(out));
+                        else
+                            k_embed<T, Tok, decltype(w)::value, false><<<grid, kBagThreads, 0, s>>>(
+                                a, static_cast<const T*>(table), tk, static_cast<T*>(out));
                     });
                 });
             }
