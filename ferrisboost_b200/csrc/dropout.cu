@@ -100,64 +100,70 @@ template <class T> __global__ void __launch_bounds__(kThreads, 4) k_dropout(cons
                 }
             continue;
         }
-        const bool odd = e & 1;
         uint64_t state = a.key + ((e >> 1) + 1) * kGamma;
-        for (uint32_t round = 0; round < a.rounds && c < a.dim; round++) {
-            uint4 lo[kAhead], hi[kAhead];
-            bool whole[kAhead];
+        // ODD: the row's units begin with the high half of a word
+        auto units = [&](auto odd, auto aligned) {
+            constexpr bool ODD = decltype(odd)::value, ALIGNED = decltype(aligned)::value;
+            for (uint32_t round = 0; round < a.rounds && c < a.dim; round++) {
+                uint4 lo[kAhead], hi[kAhead];
+                bool whole[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                whole[k] = c + k * step >= 0 && c + k * step + V <= a.dim;
-                lo[k] = *(whole[k] ? reinterpret_cast<const uint4*>(base + k * 16 * lanes) : &g_zero);
+                for (int k = 0; k < kAhead; k++) {
+                    whole[k] = c + k * step >= 0 && c + k * step + V <= a.dim;
+                    lo[k] = *(whole[k] ? reinterpret_cast<const uint4*>(base + k * 16 * lanes) : &g_zero);
+                }
+                if (!ALIGNED) {
+                    // the vector with the unit's last element: the first one again where the unit is aligned
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++)
+                        hi[k] = *(whole[k] ? reinterpret_cast<const uint4*>(base + k * 16 * lanes + (shift ? 16 : 0))
+                                           : &g_zero);
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; k++) {
+                    if (c + k * step >= a.dim) break;
+                    union {
+                        uint4 u;
+                        T v[V];
+                    } p;
+                    p.u = ALIGNED ? lo[k] : window(lo[k], hi[k], shift);
+                    if (!whole[k]) {
+#pragma unroll
+                        for (int i = 0; i < V; i++)
+                            if ((uint32_t)(c + k * step + i) < (uint32_t)a.dim) p.v[i] = from[k * step + i];
+                    }
+                    uint64_t at = state + k * stride;
+                    uint32_t half[V + 2];  // of the words from that of the first element on
+#pragma unroll
+                    for (int i = 0; i < V + ODD; i += 2) {
+                        const uint64_t w = mix64(at);
+                        half[i] = (uint32_t)w;
+                        half[i + 1] = (uint32_t)(w >> 32);
+                        at += kGamma;
+                    }
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) drop_pair(p.v + i, half[i + ODD], half[i + 1 + ODD], a);
+                    if (whole[k]) {
+                        *reinterpret_cast<uint4*>(to + k * step) = p.u;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; i++)
+                            if ((uint32_t)(c + k * step + i) < (uint32_t)a.dim) to[k * step + i] = p.v[i];
+                    }
+                }
+                c += kAhead * step;
+                from += kAhead * step;
+                to += kAhead * step;
+                base += kAhead * 16 * lanes;
+                state += kAhead * stride;
             }
-            if (!a.aligned) {
-                // the vector with the unit's last element: the first one again where the unit is aligned
-#pragma unroll
-                for (int k = 0; k < kAhead; k++)
-                    hi[k] = *(whole[k] ? reinterpret_cast<const uint4*>(base + k * 16 * lanes + (shift ? 16 : 0)) : &g_zero);
-            }
-#pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                if (c + k * step >= a.dim) break;
-                union {
-                    uint4 u;
-                    T v[V];
-                } p;
-                p.u = a.aligned ? lo[k] : window(lo[k], hi[k], shift);
-                if (!whole[k]) {
-#pragma unroll
-                    for (int i = 0; i < V; i++)
-                        if ((uint32_t)(c + k * step + i) < (uint32_t)a.dim) p.v[i] = from[k * step + i];
-                }
-                uint64_t at = state + k * stride;
-                uint32_t half[V + 1];  // of the words from that of the first element on
-#pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    const uint64_t w = mix64(at);
-                    half[i] = (uint32_t)w;
-                    half[i + 1] = (uint32_t)(w >> 32);
-                    at += kGamma;
-                }
-                if (odd) {  // the first element has the high half
-                    half[V] = (uint32_t)mix64(at);
-#pragma unroll
-                    for (int i = 0; i < V; i++) half[i] = half[i + 1];
-                }
-#pragma unroll
-                for (int i = 0; i < V; i += 2) drop_pair(p.v + i, half[i], half[i + 1], a);
-                if (whole[k]) {
-                    *reinterpret_cast<uint4*>(to + k * step) = p.u;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; i++)
-                        if ((uint32_t)(c + k * step + i) < (uint32_t)a.dim) to[k * step + i] = p.v[i];
-                }
-            }
-            c += kAhead * step;
-            from += kAhead * step;
-            to += kAhead * step;
-            base += kAhead * 16 * lanes;
-            state += kAhead * stride;
+        };
+        if (a.aligned) {
+            if (e & 1) units(std::true_type{}, std::true_type{});
+            else units(std::false_type{}, std::true_type{});
+        } else {
+            if (e & 1) units(std::true_type{}, std::false_type{});
+            else units(std::false_type{}, std::false_type{});
         }
     }
 }
