@@ -797,6 +797,33 @@ class Model:
             return classes if objective == "multi:softmax" else out
         return (1.0 / (1.0 + np.exp(-out.astype(np.float64)))).astype(np.float32)
 
+    def sample(self, data: Any, u: Any, *, temperature: Any = 1.0, top_k: Any = 0, top_p: Any = 1.0, min_p: Any = 0.0,
+               device=None) -> tuple[np.ndarray, np.ndarray]:
+        """A class drawn for each row of a multiclass model, and its probability
+        among the classes left by the limits: ``ops.sample`` of the margins with
+        ``u``, a random number in [0, 1) for each row.  A limit is a number or
+        has a value for each row.  Needs torch.  No counterpart in the reference."""
+        if self.num_outputs < 2:
+            raise ValueError("sample draws classes of a multiclass model (multi:softprob / multi:softmax)")
+        import torch
+
+        from . import ops
+        margins = self.predict(data, output_margin=True, device=device)
+        dev = torch.device("cuda", self._device(device))
+        u = np.ascontiguousarray(u, dtype=np.float32)
+        if u.shape != (len(margins),):
+            raise ValueError(f"u must have {len(margins)} values, got shape {u.shape}")
+
+        def limit(value, dtype):
+            if np.ndim(value) == 0:
+                return value
+            return torch.from_numpy(np.ascontiguousarray(value, dtype=dtype)).to(dev)
+
+        classes, probs = ops.sample(torch.from_numpy(margins).to(dev), torch.from_numpy(u).to(dev),
+                                    temperature=limit(temperature, np.float32), top_k=limit(top_k, np.int32),
+                                    top_p=limit(top_p, np.float32), min_p=limit(min_p, np.float32))
+        return classes.cpu().numpy(), probs.cpu().numpy()
+
 
 def train(params: Mapping[str, Any], data: Any, label: Any = None, num_boost_round: int = 10, weight: Any = None,
           feature_types: Sequence[str] | None = None, quiet: bool = True, header: bool = True) -> Model:
