@@ -100,17 +100,29 @@ __global__ void __launch_bounds__(kLookupThreads) k_lookup(LookupArgs a, const T
             const auto t = tokens.at(r + k * groups, 0);
             if (t < tokens.vocab) from[k] = table + t * a.table_stride;
         }
-        for (uint32_t c = lane * V; c < a.dim; c += V << a.lanes_log) {
-            P e[kLookupRows];
-#pragma unroll
-            for (int k = 0; k < kLookupRows; k++)
-                e[k] = *(from[k] ? reinterpret_cast<const P*>(from[k] + c) : reinterpret_cast<const P*>(&g_zero));
+        // narrow vectors: several slices of the columns at once, for as many bytes in flight
+        constexpr int kSlices = sizeof(P) >= 16 ? 1 : sizeof(P) >= 8 ? 2 : 4;
+        const uint32_t slice = V << a.lanes_log;
+        for (uint32_t c = lane * V; c < a.dim; c += kSlices * slice) {
+            P e[kLookupRows][kSlices];
 #pragma unroll
             for (int k = 0; k < kLookupRows; k++) {
-                Sums<V> sum;
-                sum.clear();
-                sum.add(e[k]);
-                if (to[k]) *reinterpret_cast<P*>(to[k] + c) = sum.template scaled<T>(a.scale);
+#pragma unroll
+                for (int i = 0; i < kSlices; i++)
+                    e[k][i] = *(from[k] && (kSlices == 1 || c + i * slice < a.dim)
+                                    ? reinterpret_cast<const P*>(from[k] + c + i * slice)
+                                    : reinterpret_cast<const P*>(&g_zero));
+            }
+#pragma unroll
+            for (int k = 0; k < kLookupRows; k++) {
+#pragma unroll
+                for (int i = 0; i < kSlices; i++) {
+                    Sums<V> sum;
+                    sum.clear();
+                    sum.add(e[k][i]);
+                    if (to[k] && (kSlices == 1 || c + i * slice < a.dim))
+                        *reinterpret_cast<P*>(to[k] + c + i * slice) = sum.template scaled<T>(a.scale);
+                }
             }
         }
     }

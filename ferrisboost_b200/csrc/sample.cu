@@ -360,12 +360,13 @@ __global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scor
 // a contiguous part of the places; a step is four of a lane.  Up to kSort classes
 // are sorted, and short rows take fewer bins.
 template <int WARPS, int CTAS> struct alignas(16) RowShared {
-    static constexpr int kBins = WARPS == 4 ? 256 : 1024, kSort = WARPS == 4 ? 512 : 1024, kPick = 128;
-    uint32_t low[kBins], high[kBins];     // a bin's count, or its weight as two words
+    static constexpr int kBins = WARPS == 4 ? 256 : 1024, kSort = WARPS == 4 ? 512 : 1024;
+    static constexpr int kListed = WARPS == 4 ? 64 : kSort;  // top_k up to here goes by a list: few threads sort slowly
+    static constexpr int kCount = 256;                 // lists up to here are ordered by counting
+    uint32_t low[kBins], high[kBins];     // a bin's count, or its weight as two words; then the picked keys
+    u64 all[CTAS > 1 ? kBins : 1];        // a cluster's bins
     u64 part[2][WARPS];                   // warps' partial sums; two sets, used in turn
     uint32_t found[3];                    // members of the chosen bin; of the list to sort
-    uint32_t all_key[kPick];
-    u64 all_weight[kPick];
     u64 scan[WARPS];
     u64 before, pick_above;
     uint32_t bin, pick_key, pick_same, tie_place;
@@ -379,7 +380,7 @@ template <int WARPS, int CTAS> struct alignas(16) RowShared {
 
 template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     using Sh = RowShared<WARPS, CTAS>;
-    static constexpr int kBins = Sh::kBins, kSort = Sh::kSort, kThreads = WARPS * 32, kStep = 128;
+    static constexpr int kBins = Sh::kBins, kSort = Sh::kSort, kListed = Sh::kListed, kThreads = WARPS * 32, kStep = 128;
 
     Sh& s;
     float* x;             // HELD: the block's places
@@ -560,17 +561,30 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         __syncthreads();
     }
     // After the bins are filled: the bin in which the running sum reaches the goal that goal_for(total) names
-    // (kBins: none), and the sum before it.  Every block of a cluster does the same work.
-    template <class G> __device__ __forceinline__ uint32_t find_bin(u64& before, u64& goal, G&& goal_for) {
+    // (kBins: none), and the sum before it.  With `whole` over the cluster (each block adds up its share of
+    // the bins and tells the others), else over the block.
+    template <class G> __device__ __forceinline__ uint32_t find_bin(bool whole, u64& before, u64& goal, G&& goal_for) {
         constexpr int kPer = kBins / kThreads;
-        sync_row();
+        if (CTAS > 1 && whole) {
+            sync_row();
+            constexpr int kShare = kBins / CTAS;
+            for (int i = tid; i < kShare; i += kThreads) {
+                const int b = cta * kShare + i;
+                u64 v = 0;
+#pragma unroll
+                for (int c = 0; c < CTAS; c++) v += (u64)at(s.high, c)[b] << 32 | at(s.low, c)[b];
+#pragma unroll
+                for (int c = 0; c < CTAS; c++) at(s.all, c)[b] = v;
+            }
+            sync_row();
+        } else {
+            __syncthreads();
+        }
         u64 v[kPer], mine = 0, total;
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            v[i] = 0;
-#pragma unroll
-            for (int c = 0; c < CTAS; c++)
-                v[i] += (u64)at(s.high, c)[tid * kPer + i] << 32 | at(s.low, c)[tid * kPer + i];
+            const int b = tid * kPer + i;
+            v[i] = CTAS > 1 && whole ? s.all[b] : (u64)s.high[b] << 32 | s.low[b];
             mine += v[i];
         }
         u64 run = block_before(mine, total);
@@ -602,15 +616,34 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         }
     }
 
-    // The draw from a sorted list of the row's first `members` classes, by one block; the limits end inside it.
+    // Orders s.sorted[0, members), falling: short lists by counting what is larger than each.
+    __device__ __forceinline__ void order(uint32_t members) {
+        if (members <= Sh::kCount) {
+            for (uint32_t i = tid; i < members; i += kThreads) {
+                const u64 mine = s.sorted[i];
+                uint32_t rank = 0;
+#pragma unroll 8
+                for (uint32_t j = 0; j < members; j++) rank += s.sorted[j] > mine;
+                s.sorted_weight[rank] = mine;
+            }
+            __syncthreads();
+            for (uint32_t i = tid; i < members; i += kThreads) s.sorted[i] = s.sorted_weight[i];
+            __syncthreads();
+        } else {
+            uint32_t count = Sh::kCount;
+            while (count < members) count *= 2;
+            for (uint32_t i = members + tid; i < count; i += kThreads) s.sorted[i] = 0;
+            __syncthreads();
+            sort(s.sorted, count);
+        }
+    }
+
+    // The draw from a list of the row's first `members` classes, by one block; the limits end inside it.
     __device__ __forceinline__ void draw_sorted(uint32_t members, uint64_t r, const Limits& l, float top, float u,
                                                 int32_t* out_classes, float* out_probs) {
         constexpr int kPer = kSort / kThreads;
-        uint32_t count = 32;
-        while (count < members) count *= 2;
-        for (uint32_t i = members + tid; i < count; i += kThreads) s.sorted[i] = 0;
         __syncthreads();
-        sort(s.sorted, count);
+        order(members);
         u64 item[kPer], w[kPer], mine = 0, total;
         float e[kPer];
 #pragma unroll
@@ -631,33 +664,46 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
             before += w[i];
             if (!keep) w[i] = 0;
             mine += w[i];
+            s.sorted_weight[rank] = w[i];
             // to be ordered by class: the low word is the class's complement
-            if (rank < count) {
-                s.sorted_weight[rank] = w[i];
-                s.sorted[rank] = keep ? item[i] << 32 | rank : 0;
-            }
+            s.sorted[rank] = keep ? item[i] << 32 | rank : 0;
         }
         block_before(mine, total);
-        uint32_t kept = 32;
-        while (kept < members && kept < l.top_k) kept *= 2;
+        const u64 place = place_of(u, total);
+        // what is kept is a beginning of the list: at most this many
+        const uint32_t kept = min(members, l.top_k);
+        auto win = [&](u64 run, u64 weight, uint32_t complement) {
+            if (place >= run && place < run + weight) {
+                out_classes[r] = (int32_t)~complement;
+                if (out_probs) out_probs[r] = share_of(weight, total);
+            }
+        };
         __syncthreads();
-        sort(s.sorted, kept);
+        if (kept <= Sh::kCount) {  // the weight of the lower classes, by comparing each with all
+            for (uint32_t i = tid; i < kept; i += kThreads) {
+                const u64 key = s.sorted[i];
+                u64 run = 0;
+#pragma unroll 8
+                for (uint32_t j = 0; j < kept; j++) run += s.sorted[j] > key ? s.sorted_weight[j] : 0;
+                win(run, s.sorted_weight[i], (uint32_t)(key >> 32));
+            }
+            return;
+        }
+        uint32_t count = Sh::kCount;
+        while (count < kept) count *= 2;
+        sort(s.sorted, count);
         mine = 0;
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
             const uint32_t q = tid * kPer + i;
-            item[i] = q < kept ? s.sorted[q] : 0;
+            item[i] = q < count ? s.sorted[q] : 0;
             w[i] = item[i] ? s.sorted_weight[(uint32_t)item[i]] : 0;
             mine += w[i];
         }
         u64 all, run = block_before(mine, all);
-        const u64 place = place_of(u, total);
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            if (place >= run && place < run + w[i]) {
-                out_classes[r] = (int32_t)~(uint32_t)(item[i] >> 32);
-                if (out_probs) out_probs[r] = share_of(w[i], total);
-            }
+            win(run, w[i], (uint32_t)(item[i] >> 32));
             run += w[i];
         }
     }
@@ -679,10 +725,14 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         }
         // Weights vanish 27.73 T below the maximum: bins over that span, falling, the last for the rest.
         const float per = fminf(__fmul_rn(kBins / 27.75f, l.inv_t), FLT_MAX);
-        if (!l.greedy && top < INFINITY && l.top_k < classes && l.top_k <= kSort) {
-            // At least top_k classes are at or above the top_k-th largest of the threads' maxima: those are sorted.
+        if (!l.greedy && top < INFINITY && l.top_k < classes && l.top_k <= kListed) {
+            // The classes down to a bin that holds the top_k-th of the threads' maxima (or, where there are too few
+            // threads, of all classes) are at least top_k: those are sorted.  For a short list a cluster saves
+            // the sum of its bins: each block finds the bin of its share, and the lowest of these will do.
+            const bool whole = CTAS == 1 || l.top_k > 64;
+            const uint32_t share = whole ? l.top_k : (l.top_k + CTAS - 1) / CTAS;
             clear_bins(2);
-            if (l.top_k * 4 <= kThreads * CTAS) {
+            if (share * 4 <= kThreads * (whole ? CTAS : 1)) {
                 if (most > -INFINITY) atomicAdd(&s.low[bin_of(depth(most, top, per))], 1u);
             } else {
                 each([&](float v) {
@@ -690,7 +740,8 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 });
             }
             u64 before, goal;
-            const uint32_t bin = find_bin(before, goal, [&](u64) { return (u64)l.top_k; });
+            uint32_t bin = find_bin(whole, before, goal, [&](u64) { return (u64)share; });
+            if (!whole) bin = (uint32_t)reduce(bin, 0, [](u64 a, u64 b) { return a > b ? a : b; });
             const float end = bin >= kBins - 1 ? INFINITY : bin + 0.5f;  // and what is rounded down from just there
             each_step([&](const Pack<float, 4>& p, uint32_t place) {
 #pragma unroll
@@ -751,7 +802,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                     }
                 });
                 u64 before, goal;
-                const uint32_t bin = find_bin(before, goal, [&](u64 total) -> u64 {
+                const uint32_t bin = find_bin(true, before, goal, [&](u64 total) -> u64 {
                     if (!by_weight) return l.top_k;
                     if (ties < same) total -= (same - ties) * weight_of(exp_of(cut, top, l.inv_t));
                     return goal_of(l.top_p, total);
@@ -784,53 +835,94 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                 };
                 u64 above = 0;
                 uint32_t key = 0;
-                if (members <= Sh::kPick) {  // few: each is compared with all
-                    uint32_t base = 0;
-                    for (int c = 0; c < CTAS; c++) {
-                        const uint32_t m = *at(&s.found[by_weight], c);
-                        for (uint32_t i = tid; i < m; i += kThreads) {
-                            const uint32_t k = at(list, c)[i];
-                            s.all_key[base + i] = k;
-                            s.all_weight[base + i] = weight(k);
+                auto least = [](u64 a, u64 b) { return a < b ? a : b; };
+                auto largest = [](u64 a, u64 b) { return a > b ? a : b; };
+                if (listed) {
+                    // While there are many, bins over the range of their keys leave fewer, or one key alone, as
+                    // where scores are coarse.
+                    const uint32_t* from = list;
+                    uint32_t set = by_weight, lo = 0, hi = 0xffffffffu;
+                    while (members > Sh::kCount) {
+                        const uint32_t mine = s.found[set];
+                        lo = 0xffffffffu, hi = 0;
+                        for (uint32_t i = tid; i < mine; i += kThreads) lo = min(lo, from[i]), hi = max(hi, from[i]);
+                        lo = (uint32_t)reduce(lo, 0xffffffffu, least);
+                        hi = (uint32_t)reduce(hi, 0, largest);
+                        if (lo == hi) break;
+                        int down = 0;
+                        while ((hi - lo) >> down >= kBins) down++;
+                        // the list of the bin found goes where the other limit's was, and then back
+                        const uint32_t other = set == 2 ? by_weight : 2;
+                        uint32_t* const to = s.key[other == 2 ? 1 - by_weight : by_weight];
+                        clear_bins(other);
+                        for (uint32_t i = tid; i < mine; i += kThreads) {
+                            const u64 w = weight(from[i]);
+                            const uint32_t b2 = (hi - from[i]) >> down, low = (uint32_t)w;
+                            const uint32_t old = low ? atomicAdd(&s.low[b2], low) : 0;
+                            const uint32_t high = (uint32_t)(w >> 32) + (old + low < low);
+                            if (high) atomicAdd(&s.high[b2], high);
                         }
-                        base += m;
+                        u64 front, same_goal;
+                        const uint32_t b3 = find_bin(true, front, same_goal, [&](u64) { return goal; });
+                        goal -= front;
+                        for (uint32_t i = tid; i < mine; i += kThreads) {
+                            if ((hi - from[i]) >> down == b3) to[atomicAdd(&s.found[other], 1u)] = from[i];
+                        }
+                        sync_row();
+                        members = 0;
+                        for (int c = 0; c < CTAS; c++) members += *at(&s.found[other], c);
+                        from = to;
+                        set = other;
                     }
-                    __syncthreads();
-                    for (uint32_t i = tid; i < members; i += kThreads) {
-                        const uint32_t k = s.all_key[i];
-                        u64 front = 0;
-                        uint32_t equal = 0;
-                        for (uint32_t j = 0; j < members; j++) {
-                            if (s.all_key[j] > k) front += s.all_weight[j];
-                            if (s.all_key[j] == k) equal++;
+                    if (lo == hi) {
+                        key = lo;
+                        same = members;
+                    } else {  // each compared with all
+                        uint32_t* const all_key = s.low;  // of no more use
+                        u64* const all_weight = s.sorted_weight;
+                        uint32_t base = 0;
+                        for (int c = 0; c < CTAS; c++) {
+                            const uint32_t m = *at(&s.found[set], c);
+                            for (uint32_t i = tid; i < m; i += kThreads) {
+                                const uint32_t k = at(from, c)[i];
+                                all_key[base + i] = k;
+                                all_weight[base + i] = weight(k);
+                            }
+                            base += m;
                         }
-                        if (front < goal && goal <= front + equal * s.all_weight[i]) {  // all of that key agree
-                            s.pick_key = k;
-                            s.pick_same = equal;
-                            s.pick_above = front;
+                        __syncthreads();
+                        for (uint32_t i = tid; i < members; i += kThreads) {
+                            const uint32_t k = all_key[i];
+                            u64 front = 0;
+                            uint32_t equal = 0;
+#pragma unroll 4
+                            for (uint32_t j = 0; j < members; j++) {
+                                const uint32_t other = all_key[j];
+                                front += other > k ? all_weight[j] : 0;
+                                equal += other == k;
+                            }
+                            if (front < goal && goal <= front + equal * all_weight[i]) {  // all of that key agree
+                                s.pick_key = k;
+                                s.pick_same = equal;
+                                s.pick_above = front;
+                            }
                         }
+                        __syncthreads();
+                        key = s.pick_key;
+                        same = s.pick_same;
+                        above = s.pick_above;
                     }
-                    __syncthreads();
-                    key = s.pick_key;
-                    same = s.pick_same;
-                    above = s.pick_above;
                 } else {
-                    // Many: halve the range of their keys.  All above `hi` have the weight `above`, below the
-                    // goal; with those from `lo` on it is reached.  The ends are keys that occur, so that a bin
-                    // of one score is done at once.
+                    // More than a list holds: halve the range of their keys, reading the row.  All above `hi`
+                    // have the weight `above`, below the goal; with those from `lo` on it is reached.  The ends
+                    // are keys that occur.
                     auto each_member = [&](auto&& f) {
-                        if (listed) {
-                            for (uint32_t i = tid; i < s.found[by_weight]; i += kThreads) f(list[i]);
-                        } else {
-                            each([&](float v) {
-                                if (member(v)) f(key_of(score(v)));
-                            });
-                        }
+                        each([&](float v) {
+                            if (member(v)) f(key_of(score(v)));
+                        });
                     };
                     uint32_t lo = 0xffffffffu, hi = 0;
                     each_member([&](uint32_t k) { lo = min(lo, k), hi = max(hi, k); });
-                    auto least = [](u64 a, u64 b) { return a < b ? a : b; };
-                    auto largest = [](u64 a, u64 b) { return a > b ? a : b; };
                     lo = (uint32_t)reduce(lo, 0xffffffffu, least);
                     hi = (uint32_t)reduce(hi, 0, largest);
                     while (lo < hi) {
@@ -914,30 +1006,28 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
             return sum;
         };
         // the warp's weight by eighths of its part, so that only one eighth is walked again
-        const uint32_t eighth = (steps + 7) / 8;
+        const uint32_t eighth = (steps + 7) / 8, eighths = (steps + eighth - 1) / eighth;
         u64 mine = 0, before = 0;
 #pragma unroll 1
-        for (uint32_t e = 0; e < 8; e++) {
+        for (uint32_t e = 0; e < eighths; e++) {
             u64 part = 0;
-            steps_of_warp(min(steps, e * eighth), min(steps, (e + 1) * eighth), [&](const Pack<float, 4>& p, uint32_t place) {
+            steps_of_warp(e * eighth, min(steps, (e + 1) * eighth), [&](const Pack<float, 4>& p, uint32_t place) {
                 u64 w[4];
                 part += weigh(p, place, w);
             });
             mine += part;
-            if (e * eighth < steps) {
 #pragma unroll
-                for (int d = 16; d; d /= 2) part += __shfl_xor_sync(0xffffffffu, part, d);
-            }
+            for (int d = 16; d; d /= 2) part += __shfl_xor_sync(0xffffffffu, part, d);
             if (lane == 0) s.chunk[warp][e] = part;
         }
         __syncwarp();
         const u64 total = sum(mine, &before);
         const u64 place = place_of(u[r], total);
         uint32_t e = 0;
-        while (e < 8 && place >= before && place >= before + s.chunk[warp][e]) before += s.chunk[warp][e++];
-        if (place >= before && e < 8) {  // this warp holds the class
+        while (e < eighths && place >= before && place >= before + s.chunk[warp][e]) before += s.chunk[warp][e++];
+        if (place >= before && e < eighths) {  // this warp holds the class
             u64 run = before;
-            steps_of_warp(min(steps, e * eighth), min(steps, (e + 1) * eighth), [&](const Pack<float, 4>& p, uint32_t at) {
+            steps_of_warp(e * eighth, min(steps, (e + 1) * eighth), [&](const Pack<float, 4>& p, uint32_t at) {
                 u64 w[4];
                 const u64 sum = weigh(p, at, w);
                 u64 upto = sum;
