@@ -30,22 +30,6 @@ __device__ __forceinline__ uint32_t bits_of(const DropArgs& a, uint64_t e) {
     return (uint32_t)(e & 1 ? word >> 32 : word);
 }
 
-// The 16 bytes at `shift` bytes into lo:hi, shift a multiple of 2 below 16.  All
-// units of a row have the same shift, so its words are a branch.
-__device__ __forceinline__ uint4 window(const uint4& lo, const uint4& hi, uint32_t shift) {
-    const uint32_t bits = (shift & 2) * 8;
-    auto part = [&](uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e) {
-        return make_uint4(__funnelshift_r(a, b, bits), __funnelshift_r(b, c, bits), __funnelshift_r(c, d, bits),
-                          __funnelshift_r(d, e, bits));
-    };
-    switch (shift >> 2) {
-        case 0: return part(lo.x, lo.y, lo.z, lo.w, hi.x);
-        case 1: return part(lo.y, lo.z, lo.w, hi.x, hi.y);
-        case 2: return part(lo.z, lo.w, hi.x, hi.y, hi.z);
-        default: return part(lo.w, hi.x, hi.y, hi.z, hi.w);
-    }
-}
-
 // Two elements, kept or zero.
 __device__ __forceinline__ float kept(uint32_t bits, const DropArgs& a, float v) {
     return bits >= a.threshold ? v * a.scale : 0.0f;

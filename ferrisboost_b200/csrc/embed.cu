@@ -100,28 +100,83 @@ __global__ void __launch_bounds__(kLookupThreads) k_lookup(LookupArgs a, const T
             const auto t = tokens.at(r + k * groups, 0);
             if (t < tokens.vocab) from[k] = table + t * a.table_stride;
         }
-        // narrow vectors: several slices of the columns at once, for as many bytes in flight
-        constexpr int kSlices = sizeof(P) >= 16 ? 1 : sizeof(P) >= 8 ? 2 : 4;
-        const uint32_t slice = V << a.lanes_log;
-        for (uint32_t c = lane * V; c < a.dim; c += kSlices * slice) {
-            P e[kLookupRows][kSlices];
+        for (uint32_t c = lane * V; c < a.dim; c += V << a.lanes_log) {
+            P e[kLookupRows];
+#pragma unroll
+            for (int k = 0; k < kLookupRows; k++)
+                e[k] = *(from[k] ? reinterpret_cast<const P*>(from[k] + c) : reinterpret_cast<const P*>(&g_zero));
 #pragma unroll
             for (int k = 0; k < kLookupRows; k++) {
+                Sums<V> sum;
+                sum.clear();
+                sum.add(e[k]);
+                if (to[k]) *reinterpret_cast<P*>(to[k] + c) = sum.template scaled<T>(a.scale);
+            }
+        }
+    }
+}
+
+// The same where the rows do not keep 16-byte boundaries: a lane's vectors are
+// those of the output, and each is taken from the one or two vectors of the
+// table's row that hold it.  The row's ends, partial vectors, go by element.
+template <class T, class Tok>
+__global__ void __launch_bounds__(kLookupThreads) k_lookup_odd(LookupArgs a, const T* __restrict__ table,
+                                                               Tokens<Tok> tokens, T* __restrict__ out) {
+    constexpr int V = 16 / sizeof(T), kRows = 2;
+    const uint64_t groups = (uint64_t)gridDim.x * (kLookupThreads >> a.lanes_log);
+    const uint32_t lane = threadIdx.x & ((1u << a.lanes_log) - 1);
+    const int step = V << a.lanes_log, dim = (int)a.dim;
+    for (uint64_t r = ((uint64_t)blockIdx.x * kLookupThreads + threadIdx.x) >> a.lanes_log; r < a.n;
+         r += kRows * groups) {
+        const T* from[kRows];
+        T* to[kRows];
+        int col[kRows];  // of the lane's first vector: before the row where that begins inside a vector
+        uint32_t shift[kRows];
 #pragma unroll
-                for (int i = 0; i < kSlices; i++)
-                    e[k][i] = *(from[k] && (kSlices == 1 || c + i * slice < a.dim)
-                                    ? reinterpret_cast<const P*>(from[k] + c + i * slice)
-                                    : reinterpret_cast<const P*>(&g_zero));
+        for (int k = 0; k < kRows; k++) {
+            const bool in = r + k * groups < a.n;
+            const auto t = in ? tokens.at(r + k * groups, 0) : tokens.vocab;
+            to[k] = out + (in ? r + k * groups : r) * a.out_stride;
+            col[k] = in ? (int)(lane * V) - (int)((uintptr_t)to[k] % 16 / sizeof(T)) : dim;
+            from[k] = t < tokens.vocab ? table + t * a.table_stride : nullptr;
+            shift[k] = (uint32_t)((uintptr_t)(from[k] + col[k]) % 16);
+        }
+        // up to the last vector of the row that begins furthest before its first column
+        for (int c = 0; (int)(lane * V) - (V - 1) + c < dim; c += step) {
+            uint4 lo[kRows], hi[kRows];
+#pragma unroll
+            for (int k = 0; k < kRows; k++) {
+                const bool whole = from[k] && col[k] + c >= 0 && col[k] + c + V <= dim;
+                const char* p = reinterpret_cast<const char*>(from[k] + col[k] + c) - shift[k];
+                lo[k] = *(whole ? reinterpret_cast<const uint4*>(p) : &g_zero);
+                // the vector with the last element: the first one again where it holds all
+                hi[k] = *(whole ? reinterpret_cast<const uint4*>(p + (shift[k] ? 16 : 0)) : &g_zero);
             }
 #pragma unroll
-            for (int k = 0; k < kLookupRows; k++) {
+            for (int k = 0; k < kRows; k++) {
+                const int first = col[k] + c;
+                if (first >= dim) continue;
+                union {
+                    uint4 u;
+                    Pack<T, V> p;
+                } e;
+                e.u = window(lo[k], hi[k], shift[k]);
+                const bool whole = first >= 0 && first + V <= dim;
+                if (!whole && from[k]) {
 #pragma unroll
-                for (int i = 0; i < kSlices; i++) {
-                    Sums<V> sum;
-                    sum.clear();
-                    sum.add(e[k][i]);
-                    if (to[k] && (kSlices == 1 || c + i * slice < a.dim))
-                        *reinterpret_cast<P*>(to[k] + c + i * slice) = sum.template scaled<T>(a.scale);
+                    for (int i = 0; i < V; i++)
+                        if ((uint32_t)(first + i) < (uint32_t)dim) e.p.v[i] = from[k][first + i];
+                }
+                Sums<V> sum;
+                sum.clear();
+                sum.add(e.p);
+                const Pack<T, V> o = sum.template scaled<T>(a.scale);
+                if (whole) {
+                    *reinterpret_cast<Pack<T, V>*>(to[k] + first) = o;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i++)
+                        if ((uint32_t)(first + i) < (uint32_t)dim) to[k][first + i] = o.v[i];
                 }
             }
         }
@@ -742,15 +797,22 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
             const uint32_t v = vector_width(size, dim, table, table_stride, out, out_stride), vectors = (dim + v - 1) / v;
             const Tokens<Tok> tk(tokens, token_row, token_col, vocab);
             if (per_row == 1) {
+                // rows of several 16-byte vectors that do not keep their boundaries
+                const bool odd = v * size < 16 && dim >= 64 / size && dim < 1u << 30;
                 LookupArgs a{table_stride, n, out_stride, dim, 0, scale};
-                while (1u << a.lanes_log < lanes_for(vectors)) a.lanes_log++;
-                // every SM full once, then four rows a group, then more
+                while (1u << a.lanes_log < lanes_for(odd ? dim / (16 / size) + 2 : vectors)) a.lanes_log++;
+                // every SM full once, then several rows a group, then more
                 const uint64_t wish = (n + (kLookupThreads >> a.lanes_log) - 1) / (kLookupThreads >> a.lanes_log);
                 const uint64_t full = 148 * 8;
                 const uint32_t blocks = (uint32_t)std::min<uint64_t>(
                     1u << 20, std::max(std::min(wish, full), (wish + kLookupRows - 1) / kLookupRows));
                 with_type(type, [&](auto e) {
                     using T = decltype(e);
+                    if (odd) {
+                        k_lookup_odd<T, Tok><<<blocks, kLookupThreads, 0, s>>>(a, static_cast<const T*>(table), tk,
+                                                                              static_cast<T*>(out));
+                        return;
+                    }
                     with_width<T>(v, [&](auto w) {
                         k_lookup<T, Tok, decltype(w)::value><<<blocks, kLookupThreads, 0, s>>>(
                             a, static_cast<const T*>(table), tk, static_cast<T*>(out));

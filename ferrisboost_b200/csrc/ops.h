@@ -45,6 +45,22 @@ struct Divisor {
     __device__ __forceinline__ uint32_t div(uint32_t i) const { return d <= 1 ? i : __umulhi(i, mul) >> shift; }
 };
 
+// The 16 bytes at `shift` bytes into lo:hi, shift a multiple of 2 below 16.  All
+// vectors of a row have the same shift, so its words are a branch.
+__device__ __forceinline__ uint4 window(const uint4& lo, const uint4& hi, uint32_t shift) {
+    const uint32_t bits = (shift & 2) * 8;
+    auto part = [&](uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e) {
+        return make_uint4(__funnelshift_r(a, b, bits), __funnelshift_r(b, c, bits), __funnelshift_r(c, d, bits),
+                          __funnelshift_r(d, e, bits));
+    };
+    switch (shift >> 2) {
+        case 0: return part(lo.x, lo.y, lo.z, lo.w, hi.x);
+        case 1: return part(lo.y, lo.z, lo.w, hi.x, hi.y);
+        case 2: return part(lo.z, lo.w, hi.x, hi.y, hi.z);
+        default: return part(lo.w, hi.x, hi.y, hi.z, hi.w);
+    }
+}
+
 struct Clear {
     char* p;          // rows of `bytes` bytes, `stride` bytes apart
     uint64_t rows, bytes, stride;

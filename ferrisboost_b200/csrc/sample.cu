@@ -550,7 +550,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     }
 
     // How far a score lies below the maximum, in bins.
-    __device__ __forceinline__ float depth(float v, float top, float per) { return __fmul_rn(__fsub_rn(top, v), per); }
+    __device__ __forceinline__ float depth(float v, float top, float per) { return __fmul_rn(__fsub_rn(v, top), -per); }
     // The nearest whole number by the addition of 2^23, whose low bits it becomes; monotone like the depth.
     __device__ __forceinline__ uint32_t bin_of(float d) {
         return __float_as_uint(__fadd_rn(fminf(d, kBins - 1.0f), 8388608.0f)) & (kBins - 1);
@@ -1117,9 +1117,23 @@ template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(c
                                      a.u, a.params, a.out_classes, a.out_probs));
 }
 
+// Which kernel takes a row, by its classes and the rows (us measured, both sides of each choice):
+//   up to 16     all pairs in a thread's registers: 10^6 rows of 7 f32 with top_p 27 (a warp a row: 1100)
+//   up to 256    one to eight lanes and 32 classes each: 800000 rows of 20 bf16 with top_p 103 (a warp a row:
+//                1390); fewer lanes a row, fewer rounds
+//   up to 8192   a block, the row in shared memory: 2048 rows of 1000 f16 with top_p 25 (32 lanes of 32
+//                classes: 44)
+//   longer       a batch: a block, the row read again from the L2 for each step: 256 rows of 131071 bf16 with
+//                top_k 50 31 (a cluster each, in shared memory: 310).  1024 threads where every SM has at most one
+//                row (148 rows with top_p: 103 against 148) or where rows differ in work and the longest one counts
+//                (256 rows with limits of their own: 143 against 162), else two rows an SM (256 rows with top_p: 186
+//                against 202);
+//                a few rows: eight SMs share each, 1 row of 128000 f32 with top_k 50 16.
 template <class T> void launch_sample(const SampleArgs& a) {
     count_launch();
     const uint32_t k = a.classes;
+    const auto& p = a.params;
+    const bool unequal = p.temperatures || p.top_ks || p.top_ps || p.min_ps;
     if (k <= 2) launch_thread<T, 2>(a);
     else if (k <= 3) launch_thread<T, 3>(a);
     else if (k <= 4) launch_thread<T, 4>(a);
@@ -1137,6 +1151,7 @@ template <class T> void launch_sample(const SampleArgs& a) {
     else if (k <= 256) launch_lanes<T, 8, 32>(a);
     else if (k <= 2048) launch_row<T, true, 4, 1, 8>(a);
     else if (k <= 8192) launch_row<T, true, 8, 1, 3>(a);
+    else if (a.n >= 64 && a.n <= (unequal ? 296 : 148)) launch_row<T, false, 32, 1, 1>(a);
     else if (a.n >= 64) launch_row<T, false, 16, 1, 2>(a);
     else if (k <= 262144) launch_row<T, true, 16, 8, 1>(a);  // 32768 scores of a block: 128 KB
     else launch_row<T, false, 16, 8, 1>(a);

@@ -484,3 +484,34 @@ def test_sample_temperatures_at_the_ends_of_f32(K):
             kept = x.argsort(dim=1, descending=True, stable=True)[:, :450].sort(1).values
             want = kept.gather(1, (u.double() * 450).long()[:, None])[:, 0]
             assert torch.equal(c.long(), want) and torch.allclose(p, torch.full_like(p, 1 / 450), rtol=2.0 ** -23)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dim", [16, 31, 32, 33, 63, 65, 201, 1023, 2051])
+def test_lookup_of_rows_off_16_byte_boundaries(dim, dtype):
+    """One token a row: the same bits as indexing, at every distance of table
+    and output from a 16-byte boundary, and nothing outside the rows is written."""
+    n, vocab = 67, 29
+    for tshift, tpad, oshift, opad in ((0, 0, 0, 0), (1, 0, 0, 0), (0, 1, 3, 0), (5, 7, 2, 1), (0, 0, 1, 2), (3, 5, 3, 5)):
+        table = randn((tshift + vocab * (dim + tpad),), dim, dtype)[tshift:].view(vocab, dim + tpad)[:, :dim]
+        tok = tokens_of(n, 1, vocab, dim)[:, 0]
+        flat = torch.full((oshift + n * (dim + opad) + 9,), 9.0, dtype=dt(dtype), device="cuda")
+        out = flat[oshift:oshift + n * (dim + opad)].view(n, dim + opad)[:, :dim]
+        ops().embed(table, tok, scale=2.0, out=out)
+        found = (tok >= 0) & (tok < vocab)
+        want = torch.where(found[:, None], table[tok.clamp(0, vocab - 1).long()].float() * 2, 0.0).to(dt(dtype))
+        assert torch.equal(out, want)
+        spare = flat.clone()
+        spare[oshift:oshift + n * (dim + opad)].view(n, dim + opad)[:, :dim] = 9.0
+        assert (spare == 9.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n,dim", [(20011, 201), (60001, 37), (150001, 64), (200003, 5)])
+def test_lookup_of_many_rows(n, dim, dtype):
+    """More rows than groups: each group takes several, bits as by indexing."""
+    table = randn((4000, dim), 1, dtype)
+    tok = tokens_of(n, 1, 4000, 2, "int64")[:, 0]
+    found = (tok >= 0) & (tok < 4000)
+    want = torch.where(found[:, None], table[tok.clamp(0, 3999)].float() * 0.5, 0.0).to(dt(dtype))
+    assert torch.equal(ops().embed(table, tok, scale=0.5), want)
