@@ -3,10 +3,12 @@
 // A class of score x weighs w = floor(2^40 exp((x - max) / T)).  Every limit
 // keeps a beginning of the order (score falling, equal scores by class), so
 // what is kept is "every class above a threshold score, and the first `ties`
-// classes of that score"; the threshold is found by counting and summing
-// weights per digit of an ordered key, not by sorting.  Sums of weights are
-// 64-bit whole numbers: 2^20 classes of at most 2^40 fit, and no order of
-// additions changes them.
+// classes of that score": the threshold is found, and the row is not sorted
+// (only the few candidates of a small top_k are).  Sums of weights are 64-bit
+// whole numbers: 2^20 classes of at most 2^40 fit, and no order of additions
+// changes them, so every kernel below gives the same draw.  2^-40 of the first
+// class's weight is the unit because the products by 2^40 are exact in f32 and
+// the sums of 2^20 classes fit; what is less is never drawn.
 #include <cfloat>
 
 #include <cooperative_groups.h>
@@ -72,7 +74,9 @@ __device__ __forceinline__ float share_of(u64 w, u64 total) {
 
 // ------------------------------------------------------- a thread per row
 // Up to KP classes in registers.  A class's place in the order and the weight
-// before it come from comparing each pair once.
+// before it come from comparing all pairs.  10^6 rows of 7 f32 with top_p 0.9: 27 us
+// (1.5 TB/s; 17 without top_p), bound by the issue of about 560 operations for 32
+// rows.
 template <class T, int KP>
 __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ scores, uint64_t n, uint32_t classes,
                                                        uint64_t stride, const float* __restrict__ u,

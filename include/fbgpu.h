@@ -444,7 +444,8 @@ fbgpu_status fbgpu_explain_device(fbgpu_model* m, int32_t kind, const float* X, 
  * `dim` elements of `type`, summed in f32 and rounded once.  Token (r, j) is at
  * tokens + r * token_row + j * token_col; one outside [0, vocab) stands for a
  * missing value and adds nothing (a row of only such tokens is zero).  The
- * order of the sum depends on the sizes alone. */
+ * order of the sum depends on the sizes alone.  With several tokens a row, dim
+ * is at most 2097120. */
 fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vocab, uint32_t dim, uint64_t table_stride,
                          const void* tokens, int32_t token_type, uint64_t n, uint32_t per_row, uint64_t token_row,
                          uint64_t token_col, float scale, void* out, uint64_t out_stride, void* stream);
@@ -479,7 +480,7 @@ fbgpu_status fbgpu_dropout(const void* x, int32_t type, uint64_t n, uint64_t dim
  * maximum.  top_k 0, top_p 1 and min_p 0 are no limit.  Values of an array
  * outside the ranges are read so: a temperature that is not above 0 as 0, a top_k
  * below 1 as none, top_p below 0 as 0 and NaN as 1, min_p above 1 as 1 and NaN
- * as 0. */
+ * as 0.  A temperature above 0 is taken as at least 2^-126. */
 typedef struct fbgpu_sample_params {
     float temperature;  /* >= 0 */
     int32_t top_k;      /* >= 0 */
