@@ -10,8 +10,9 @@ The functions take torch CUDA tensors (float32, float16 or bfloat16) and return
 new ones, or fill ``out``.  Like torch's own operations they are enqueued on the
 current stream of the tensors' device and do not wait for it; a tensor made on
 another stream needs the usual ``wait_stream`` / ``record_stream``.  They can be
-captured into a CUDA graph.  Wrong arguments raise ValueError before anything
-is enqueued.  The kernels are ``fbgpu_embed``, ``fbgpu_embed_grad``,
+captured into a CUDA graph.  They do not record gradients: a training step calls
+the backward operators itself (examples/leaf_head.py).  Wrong arguments raise
+ValueError before anything is enqueued.  The kernels are ``fbgpu_embed``, ``fbgpu_embed_grad``,
 ``fbgpu_dropout`` and ``fbgpu_sample`` of include/fbgpu.h, which has the exact
 definitions; there is no CPU path.
 """
@@ -31,7 +32,7 @@ _F32 = {torch.float32: 0}
 _TOKENS = {torch.int32: 0, torch.int64: 1}                        # FBGPU_I32, FBGPU_I64
 
 
-_lib_ = _lib.load()
+_entry = _lib.load()
 _device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
@@ -77,7 +78,7 @@ def _call(device: int, f: Any, *args: Any) -> None:
         with torch.cuda.device(device):
             status = f(*args, _stream(device))
     if status:
-        message = (_lib_.fbgpu_last_error(None) or b"").decode()
+        message = (_entry.fbgpu_last_error(None) or b"").decode()
         raise (ValueError if status == 1 else RuntimeError)(message)
 
 
@@ -115,7 +116,7 @@ def embed(table: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0,
     vocab, dim = table.shape
     _count(dim, k)
     out = table.new_empty((n, dim)) if out is None else _out(out, (n, dim), table)
-    _call(device, _lib_.fbgpu_embed, table.data_ptr(), code, vocab, dim, _rows("table", table), tokens.data_ptr(), tcode, n,
+    _call(device, _entry.fbgpu_embed, table.data_ptr(), code, vocab, dim, _rows("table", table), tokens.data_ptr(), tcode, n,
           k, trow, tcol, scale, out.data_ptr(), _rows("out", out))
     return out
 
@@ -141,9 +142,9 @@ def embed_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale: f
     dim = grad.shape[1]
     _count(dim, k)
     out = grad.new_empty((vocab, dim)) if out is None else _out(out, (vocab, dim), grad)
-    size = _lib_.fbgpu_embed_grad_workspace(n, k, vocab, dim)
+    size = _entry.fbgpu_embed_grad_workspace(n, k, vocab, dim)
     space = grad.new_empty(size, dtype=torch.uint8)
-    _call(device, _lib_.fbgpu_embed_grad, grad.data_ptr(), code, n, k, dim, _rows("grad", grad), tokens.data_ptr(), tcode,
+    _call(device, _entry.fbgpu_embed_grad, grad.data_ptr(), code, n, k, dim, _rows("grad", grad), tokens.data_ptr(), tcode,
           trow, tcol, vocab, scale, out.data_ptr(), _rows("out", out), space.data_ptr(), size)
     return out
 
@@ -170,7 +171,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, *,
     else:
         raise ValueError(f"x and out must be contiguous, or 2-D with contiguous rows; x has shape {tuple(x.shape)} "
                          f"and strides {x.stride()}")
-    _call(x.get_device(), _lib_.fbgpu_dropout, x.data_ptr(), code, n, dim, xs, p, seed & 0xFFFFFFFFFFFFFFFF,
+    _call(x.get_device(), _entry.fbgpu_dropout, x.data_ptr(), code, n, dim, xs, p, seed & 0xFFFFFFFFFFFFFFFF,
           offset & 0xFFFFFFFFFFFFFFFF, out.data_ptr(), os)
     return out
 
@@ -228,6 +229,6 @@ def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: Any = 1.0, top
     classes = u.new_empty(n, dtype=torch.int32) if classes is None else _result("classes", classes, u, torch.int32)
     probs = u.new_empty(n) if probs is None else _result("probs", probs, u, torch.float32)
     params = _lib.FbgpuSampleParams(t, int(tk), tp, mp, ts, tks, tps, mps)
-    _call(device, _lib_.fbgpu_sample, scores.data_ptr(), code, n, k, _rows("scores", scores), u.data_ptr(),
+    _call(device, _entry.fbgpu_sample, scores.data_ptr(), code, n, k, _rows("scores", scores), u.data_ptr(),
           C.byref(params), classes.data_ptr(), probs.data_ptr())
     return classes, probs

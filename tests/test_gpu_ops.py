@@ -450,6 +450,52 @@ def test_ops_run_on_the_current_stream_and_in_a_graph():
     assert torch.equal(out[0], want[0] * 2) and torch.equal(out[3], want[3])
 
 
+def test_large_forms_in_a_graph_follow_new_inputs():
+    """The sort in several launches, a cluster per row and a block per row,
+    captured once and replayed on other tokens and scores."""
+    n, k, vocab = 30000, 4, 3000
+    tok, grad = tokens_of(n, k, vocab, 1), randn((n, 20), 2)
+    scores = [randn((2, 70000), 3), randn((80, 5000), 4), randn((70, 20001), 5, "bfloat16")]
+    u = [torch.rand(len(x), generator=gen(6), device="cuda") for x in scores]
+
+    def step():
+        return [ops().embed_grad(grad, tok, vocab)] + [
+            ops().sample(x, r, top_k=k_, top_p=0.9)[0] for x, r in zip(scores, u) for k_ in (0, 30)]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (7, 8):
+        tok.copy_(tokens_of(n, k, vocab, seed))
+        for i, x in enumerate(scores):
+            x.copy_(randn(x.shape, seed + i, str(x.dtype)[6:]))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_two_streams_at_once():
+    """Calls on two streams do not share anything."""
+    tok = [tokens_of(40000, 3, 900, s) for s in (1, 2)]
+    grad = [randn((40000, 24), s) for s in (3, 4)]
+    x = [randn((4, 40000), s) for s in (5, 6)]
+    u = torch.rand(4, generator=gen(7), device="cuda")
+    want = [(ops().embed_grad(g, t, 900), ops().sample(s, u, top_p=0.7)[0]) for g, t, s in zip(grad, tok, x)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append((ops().embed_grad(grad[i], tok[i], 900), ops().sample(x[i], u, top_p=0.7)[0]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
+
+
 def test_launches_are_counted():
     from ferrisboost_b200 import _lib
     before = _lib.load().fbgpu_launch_count()
