@@ -364,8 +364,8 @@ __global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scor
 // a contiguous part of the places; a step is four of a lane.  Up to kSort classes
 // are sorted, and short rows take fewer bins.
 template <int WARPS, int CTAS> struct alignas(16) RowShared {
-    static constexpr int kBins = WARPS == 4 ? 256 : 1024, kSort = WARPS == 4 ? 512 : 1024;
-    static constexpr int kListed = WARPS == 4 ? 64 : kSort;  // top_k up to here goes by a list: few threads sort slowly
+    static constexpr int kBins = WARPS <= 4 ? 256 : 1024, kSort = WARPS <= 2 ? 256 : WARPS == 4 ? 512 : 1024;
+    static constexpr int kListed = WARPS <= 4 ? 64 : kSort;  // top_k up to here goes by a list: few threads sort slowly
     static constexpr int kCount = 256;                 // lists up to here are ordered by counting
     uint32_t low[kBins], high[kBins];     // a bin's count, or its weight as two words; then the picked keys
     u64 all[CTAS > 1 ? kBins : 1];        // a cluster's bins
@@ -1125,8 +1125,10 @@ template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(c
 //   up to 16     all pairs in a thread's registers: 10^6 rows of 7 f32 with top_p 27 (a warp a row: 1100)
 //   up to 256    one to eight lanes and 32 classes each: 800000 rows of 20 bf16 with top_p 103 (a warp a row:
 //                1390); fewer lanes a row, fewer rounds
-//   up to 8192   a block, the row in shared memory: 2048 rows of 1000 f16 with top_p 25 (32 lanes of 32
-//                classes: 44)
+//   up to 8192   a block, the row in shared memory: 2048 rows of 1000 f16 with top_p 20 (32 lanes of 32
+//                classes: 44).  Many short rows take blocks of one or two warps, so that all are resident
+//                (8000 rows of 300 bf16 with top_p 39 with one warp, 47 with two, 63 with four; 2048 of 1000
+//                25, 21, 25), few rows four, for their latency (512 rows of 1000: 23, 17, 13)
 //   longer       a batch: a block, the row read again from the L2 for each step: 256 rows of 131071 bf16 with
 //                top_k 50 31 (a cluster each, in shared memory: 310).  1024 threads where every SM has at most one
 //                row (148 rows with top_p: 103 against 148) or where rows differ in work and the longest one counts
@@ -1153,6 +1155,8 @@ template <class T> void launch_sample(const SampleArgs& a) {
     else if (k <= 64) launch_lanes<T, 2, 32>(a);
     else if (k <= 128) launch_lanes<T, 4, 32>(a);
     else if (k <= 256) launch_lanes<T, 8, 32>(a);
+    else if (k <= 512 && a.n >= 2048) launch_row<T, true, 1, 1, 20>(a);
+    else if (k <= 2048 && a.n >= 1024) launch_row<T, true, 2, 1, 16>(a);
     else if (k <= 2048) launch_row<T, true, 4, 1, 8>(a);
     else if (k <= 8192) launch_row<T, true, 8, 1, 3>(a);
     else if (a.n >= 64 && a.n <= (unequal ? 296 : 148)) launch_row<T, false, 32, 1, 1>(a);

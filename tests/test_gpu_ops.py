@@ -518,6 +518,22 @@ def test_sample_at_the_edges_of_the_variants(K):
             assert torch.equal(c64, c.repeat(40)) and torch.equal(p64, p.repeat(40))
 
 
+@pytest.mark.parametrize("K", [257, 300, 512, 513, 1000, 2048])
+def test_sample_batches_equal_few_rows(K):
+    """Large batches of short rows take smaller blocks: the same draws."""
+    x = 2 * randn((40, K), K, "float16")
+    x[3] = 1.0
+    x[4] = torch.round(x[4])
+    x[5] = -math.inf
+    u = torch.rand(40, generator=gen(K), device="cuda")
+    for limits in LIMITS + [(0.9, 200, 0.95, 0.0), (50.0, 0, 0.6, 0.0)]:
+        c, p = check_draw(x, u, *limits)
+        for times in (30, 60):
+            cm, pm = ops().sample(x.repeat(times, 1), u.repeat(times), temperature=limits[0], top_k=limits[1],
+                                  top_p=limits[2], min_p=limits[3])
+            assert torch.equal(cm, c.repeat(times)) and torch.equal(pm, p.repeat(times))
+
+
 @pytest.mark.parametrize("K", [700, 3000, 40000])
 def test_sample_temperatures_at_the_ends_of_f32(K):
     x = randn((4, K), K)
