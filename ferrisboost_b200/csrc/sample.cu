@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scor
 
 // ------------------------------------------------- a block or cluster per row
 // WARPS warps of CTAS blocks (one cluster) hold a row.  Its scores are brought
-// into shared memory as f32 once (HELD; other rows are read again for every
+// into shared memory once (HELD; other rows are read again for every
 // step, from the L2) and every later step is a short loop over them: held in
 // registers, the unrolled steps ran out of the instruction cache.  Places are
 // counted from the 16-byte boundary at or before the row's first class, so that
@@ -387,7 +387,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     static constexpr int kBins = Sh::kBins, kSort = Sh::kSort, kListed = Sh::kListed, kThreads = WARPS * 32, kStep = 128;
 
     Sh& s;
-    float* x;             // HELD: the block's places
+    T* x;                 // HELD: the block's places
     const T* row;
     uint32_t classes, shift;
     uint32_t steps;       // of a warp
@@ -395,7 +395,7 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     int lane, warp, tid, cta, parity = 0;
     float most;           // HELD: the largest score that this thread brought
 
-    __device__ __forceinline__ RowDraw(Sh& sh, float* held, uint32_t steps_) : s(sh), x(held), steps(steps_) {
+    __device__ __forceinline__ RowDraw(Sh& sh, T* held, uint32_t steps_) : s(sh), x(held), steps(steps_) {
         lane = threadIdx.x & 31;
         warp = threadIdx.x >> 5;
         tid = threadIdx.x;
@@ -443,18 +443,13 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
             for (int k = 0; k < kAhead; k++) {
                 const uint32_t v = v0 + k * kThreads, place = block_first + v * V;
                 if (v >= vectors) break;
-                float f[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) f[i] = to_f32(p[k].v[i]);
                 if (!inside(place, V)) {
 #pragma unroll
-                    for (int i = 0; i < V; i++) f[i] = one(place + i);
+                    for (int i = 0; i < V; i++) p[k].v[i] = from_f32<T>(one(place + i));
                 }
 #pragma unroll
-                for (int i = 0; i < V; i++) most = fmaxf(most, f[i]);
-#pragma unroll
-                for (int i = 0; i < V; i += 4)
-                    *reinterpret_cast<float4*>(x + v * V + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                for (int i = 0; i < V; i++) most = fmaxf(most, to_f32(p[k].v[i]));
+                *reinterpret_cast<uint4*>(x + v * V) = p[k].u;
             }
         }
         __syncthreads();
@@ -462,10 +457,15 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
     // f(four scores, place of the first) for the lane's steps [from, to), in order.  A score may be NaN.
     template <class F> __device__ __forceinline__ void steps_of_warp(uint32_t from, uint32_t to, F&& f) {
         if (HELD) {
-            const float* mine = x + (warp_first - block_first) + lane * 4;
+            const T* mine = x + (warp_first - block_first) + lane * 4;
 #pragma unroll 2
-            for (uint32_t i = from; i < to; i++)
-                f(*reinterpret_cast<const Pack<float, 4>*>(mine + i * kStep), warp_first + i * kStep + lane * 4);
+            for (uint32_t i = from; i < to; i++) {
+                const Pack<T, 4> q = *reinterpret_cast<const Pack<T, 4>*>(mine + i * kStep);
+                Pack<float, 4> p;
+#pragma unroll
+                for (int j = 0; j < 4; j++) p.v[j] = to_f32(q.v[j]);
+                f(p, warp_first + i * kStep + lane * 4);
+            }
             return;
         }
         constexpr int kAhead = 4;
@@ -1063,7 +1063,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS)
                  float* __restrict__ out_probs) {
     using Sh = RowShared<WARPS, CTAS>;
     extern __shared__ __align__(16) unsigned char memory[];
-    RowDraw<T, HELD, WARPS, CTAS> d(*reinterpret_cast<Sh*>(memory), reinterpret_cast<float*>(memory + sizeof(Sh)), steps);
+    RowDraw<T, HELD, WARPS, CTAS> d(*reinterpret_cast<Sh*>(memory), reinterpret_cast<T*>(memory + sizeof(Sh)), steps);
     for (uint64_t r = blockIdx.x / CTAS; r < n; r += gridDim.x / CTAS) {
         d.open(scores + r * stride, classes);
         d.draw(r, params, u, out_classes, out_probs);
@@ -1102,7 +1102,7 @@ template <class T> uint32_t steps_of(uint32_t classes, uint32_t warps) {
 template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(const SampleArgs& a) {
     using Sh = RowShared<WARPS, CTAS>;
     const uint32_t steps = steps_of<T>(a.classes, WARPS * CTAS);
-    const size_t bytes = sizeof(Sh) + (HELD ? (size_t)WARPS * steps * 128 * 4 : 0);
+    const size_t bytes = sizeof(Sh) + (HELD ? (size_t)WARPS * steps * 128 * sizeof(T) : 0);
     const auto kernel = k_sample_row<T, HELD, WARPS, CTAS, BLOCKS>;
     if (bytes > 48 << 10)
         FB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
@@ -1158,10 +1158,10 @@ template <class T> void launch_sample(const SampleArgs& a) {
     else if (k <= 512 && a.n >= 2048) launch_row<T, true, 1, 1, 20>(a);
     else if (k <= 2048 && a.n >= 1024) launch_row<T, true, 2, 1, 16>(a);
     else if (k <= 2048) launch_row<T, true, 4, 1, 8>(a);
-    else if (k <= 8192) launch_row<T, true, 8, 1, 3>(a);
+    else if (k <= 8192) launch_row<T, true, 8, 1, 4>(a);
     else if (a.n >= 64 && a.n <= (unequal ? 296 : 148)) launch_row<T, false, 32, 1, 1>(a);
     else if (a.n >= 64) launch_row<T, false, 16, 1, 2>(a);
-    else if (k <= 262144) launch_row<T, true, 16, 8, 1>(a);  // 32768 scores of a block: 128 KB
+    else if (k <= 262144) launch_row<T, true, 16, 8, 1>(a);  // 32768 scores of a block: up to 128 KB
     else launch_row<T, false, 16, 8, 1>(a);
 }
 
