@@ -732,8 +732,9 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
         if (!l.greedy && top < INFINITY && l.top_k < classes && l.top_k <= kListed) {
             // The classes down to a bin that holds the top_k-th of the threads' maxima (or, where there are too few
             // threads, of all classes) are at least top_k: those are sorted.  For a short list a cluster saves
-            // the sum of its bins: each block finds the bin of its share, and the lowest of these will do.
-            const bool whole = CTAS == 1 || l.top_k > 64;
+            // the sum of its bins: each block finds the bin of its share, and the lowest of these will do.  (Not for
+            // 16-bit scores, whose many equal ones make that list long.)
+            const bool whole = CTAS == 1 || l.top_k > 64 || sizeof(T) == 2;
             const uint32_t share = whole ? l.top_k : (l.top_k + CTAS - 1) / CTAS;
             clear_bins(2);
             if (share * 4 <= kThreads * (whole ? CTAS : 1)) {
@@ -1129,12 +1130,13 @@ template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(c
 //                classes: 44).  Many short rows take blocks of one or two warps, so that all are resident
 //                (8000 rows of 300 bf16 with top_p 39 with one warp, 47 with two, 63 with four; 2048 of 1000
 //                25, 21, 25), few rows four, for their latency (512 rows of 1000: 23, 17, 13)
-//   longer       a batch: a block, the row read again from the L2 for each step: 256 rows of 131071 bf16 with
-//                top_k 50 31 (a cluster each, in shared memory: 310).  1024 threads where every SM has at most one
+//   longer       a batch: a block, up to 64 KB of row in shared memory (1000 rows of 20000 bf16 with top_p 117; read
+//                again from the L2 for each step 133), longer ones read again: 256 rows of 131071 bf16 with top_k
+//                50 31 (a cluster each, in shared memory: 310).  1024 threads where every SM has at most one
 //                row (148 rows with top_p: 103 against 148) or where rows differ in work and the longest one counts
-//                (256 rows with limits of their own: 143 against 162), else two rows an SM (256 rows with top_p: 186
+//                (256 rows with limits of their own: 144 against 162), else two rows an SM (256 rows with top_p: 186
 //                against 202);
-//                a few rows: eight SMs share each, 1 row of 128000 f32 with top_k 50 16.
+//                a few rows: eight SMs share each, 1 row of 128000 f32 with top_k 50 15.
 template <class T> void launch_sample(const SampleArgs& a) {
     count_launch();
     const uint32_t k = a.classes;
@@ -1159,7 +1161,9 @@ template <class T> void launch_sample(const SampleArgs& a) {
     else if (k <= 2048 && a.n >= 1024) launch_row<T, true, 2, 1, 16>(a);
     else if (k <= 2048) launch_row<T, true, 4, 1, 8>(a);
     else if (k <= 8192) launch_row<T, true, 8, 1, 4>(a);
-    else if (a.n >= 64 && a.n <= (unequal ? 296 : 148)) launch_row<T, false, 32, 1, 1>(a);
+    else if (a.n >= 64 && a.n <= 148) launch_row<T, false, 32, 1, 1>(a);
+    else if (a.n >= 64 && k * sizeof(T) <= 65536) launch_row<T, true, 16, 1, 2>(a);
+    else if (a.n >= 64 && a.n <= 296 && unequal) launch_row<T, false, 32, 1, 1>(a);
     else if (a.n >= 64) launch_row<T, false, 16, 1, 2>(a);
     else if (k <= 262144) launch_row<T, true, 16, 8, 1>(a);  // 32768 scores of a block: up to 128 KB
     else launch_row<T, false, 16, 8, 1>(a);
