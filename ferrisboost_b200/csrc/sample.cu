@@ -1136,7 +1136,9 @@ template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(c
 //                row (148 rows with top_p: 103 against 148) or where rows differ in work and the longest one counts
 //                (256 rows with limits of their own: 144 against 162), else two rows an SM (256 rows with top_p: 186
 //                against 202);
-//                a few rows: eight SMs share each, 1 row of 128000 f32 with top_k 50 15.
+//                up to 8 rows of more than 32768: eight SMs share each, 1 row of 128000 f32 with top_k 50 15; 8 rows
+//                of 131071 bf16 with top_p 47 (a block each: 101), 16 rows with top_k 50 29 (23), as not all of 16
+//                such clusters run at a time; 18 rows of 20000 with top_p 43 (27).
 template <class T> void launch_sample(const SampleArgs& a) {
     count_launch();
     const uint32_t k = a.classes;
@@ -1161,12 +1163,12 @@ template <class T> void launch_sample(const SampleArgs& a) {
     else if (k <= 2048 && a.n >= 1024) launch_row<T, true, 2, 1, 16>(a);
     else if (k <= 2048) launch_row<T, true, 4, 1, 8>(a);
     else if (k <= 8192) launch_row<T, true, 8, 1, 4>(a);
-    else if (a.n >= 64 && a.n <= 148) launch_row<T, false, 32, 1, 1>(a);
-    else if (a.n >= 64 && k * sizeof(T) <= 65536) launch_row<T, true, 16, 1, 2>(a);
-    else if (a.n >= 64 && a.n <= 296 && unequal) launch_row<T, false, 32, 1, 1>(a);
-    else if (a.n >= 64) launch_row<T, false, 16, 1, 2>(a);
-    else if (k <= 262144) launch_row<T, true, 16, 8, 1>(a);  // 32768 scores of a block: up to 128 KB
-    else launch_row<T, false, 16, 8, 1>(a);
+    else if (k > 32768 && a.n <= 8 && k <= 262144) launch_row<T, true, 16, 8, 1>(a);  // up to 128 KB a block
+    else if (k > 32768 && a.n <= 8) launch_row<T, false, 16, 8, 1>(a);
+    else if (a.n <= 148) launch_row<T, false, 32, 1, 1>(a);
+    else if (k * sizeof(T) <= 65536) launch_row<T, true, 16, 1, 2>(a);
+    else if (a.n <= 296 && unequal) launch_row<T, false, 32, 1, 1>(a);
+    else launch_row<T, false, 16, 1, 2>(a);
 }
 
 }  // namespace
