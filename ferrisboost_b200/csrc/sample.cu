@@ -43,8 +43,9 @@ __device__ __forceinline__ Limits limits_of(const fbgpu_sample_params& p, uint64
     return l;
 }
 
-// -0 as +0 (they are equal scores) and NaN as -infinity.
-__device__ __forceinline__ float score(float x) { return x == x ? __fadd_rn(x, 0.0f) : -INFINITY; }
+// NaN as -infinity; where scores become keys, also -0 as +0 (they are equal scores).
+__device__ __forceinline__ float ruled(float x) { return fmaxf(x, -INFINITY); }
+__device__ __forceinline__ float score(float x) { return __fadd_rn(ruled(x), 0.0f); }
 // Unsigned order of the scores.
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t b = __float_as_uint(x);
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
         float x[KP], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < KP; i++) {
-            x[i] = i < classes ? score(to_f32(row[i])) : -INFINITY;
+            x[i] = i < classes ? ruled(to_f32(row[i])) : -INFINITY;
             top = fmaxf(top, x[i]);
         }
         int32_t drawn = -1;
@@ -105,12 +106,12 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
                 top = 0.0f;
             }
             u64 w[KP];
-            uint32_t keep = 0;
+            uint32_t keep = ~0u;
 #pragma unroll
             for (int i = 0; i < KP; i++) {
                 const float e = exp_of(x[i], top, l.inv_t);
                 w[i] = weight_of(e);
-                if (!(e < l.min_p)) keep |= 1u << i;
+                if (l.min_p > 0.0f && e < l.min_p) keep &= ~(1u << i);
             }
             u64 sum = 0;
             if (l.top_k < classes) {
@@ -147,11 +148,11 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
 #pragma unroll
             for (int i = 0; i < KP; i++) total += w[i] = keep >> i & 1 ? w[i] : 0;
             const u64 place = place_of(u[r], total);
-            u64 run = total, won = 0;
+            u64 run = 0, won = 0;
 #pragma unroll
-            for (int i = KP - 1; i >= 0; i--) {
-                run -= w[i];
-                if (run <= place && place < run + w[i]) drawn = i, won = w[i];
+            for (int i = 0; i < KP; i++) {
+                run += w[i];
+                if (run > place && drawn < 0) drawn = i, won = w[i];
             }
             share = share_of(won, total);
         }
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(128) k_sample_thread(const T* __restrict__ sco
 }
 
 // -------------------------------------------------- a few lanes of a warp per row
-// L lanes (1 to 32) hold a row in registers, lane l the classes [E * l, E * l + E).
+// L lanes (1 to 8) hold a row in registers, lane l the classes [E * l, E * l + E).
 // A limit's threshold is found by halving the range of scores it lies in: each
 // round sums what is at or above the middle, and the range's new end is the
 // nearest score on its side of the middle, so that about log2(classes) rounds
@@ -193,13 +194,13 @@ __global__ void __launch_bounds__(128) k_sample_lanes(const T* __restrict__ scor
         __syncwarp();
         if (L == 1) {
             const T* row = scores + r * stride;
-            for (int c = 0; c < E; c++) own[c] = c < classes ? score(to_f32(row[c])) : -INFINITY;
+            for (int c = 0; c < E; c++) own[c] = c < classes ? ruled(to_f32(row[c])) : -INFINITY;
         } else {
             const T* row = scores + r * stride;
 #pragma unroll 4
             for (int c = lane; c < L * E; c += L) {
                 float* to = own + (c / E - lane) * (E + 1) + c % E;
-                *to = c < classes ? score(to_f32(row[c])) : -INFINITY;
+                *to = c < classes ? ruled(to_f32(row[c])) : -INFINITY;
             }
         }
         __syncwarp();
