@@ -1133,7 +1133,7 @@ template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(c
 
 // Which kernel takes a row, by its classes and the rows (us measured, both sides of each choice):
 //   up to 16     all pairs in a thread's registers: 10^6 rows of 7 f32 with top_p 27 (a warp a row: 1100)
-//   up to 256    one to eight lanes and 32 classes each: 800000 rows of 20 bf16 with top_p 103 (a warp a row:
+//   up to 256    one to eight lanes and 32 classes each: 800000 rows of 20 bf16 with top_p 100 (a warp a row:
 //                1390); fewer lanes a row, fewer rounds
 //   up to 8192   a block, the row in shared memory: 2048 rows of 1000 f16 with top_p 20 (32 lanes of 32
 //                classes: 44).  Many short rows take blocks of one or two warps, so that all are resident
