@@ -586,28 +586,47 @@ template <class T, int V> __device__ __forceinline__ void write_row(const RunSum
     *reinterpret_cast<Pack<T, V>*>(out + key * a.out_stride + c) = sum.template scaled<T>(a.scale);
 }
 
-template <class T, int V>
+template <class T, int V, int M>  // M vectors of a lane, lanes apart
 __global__ void __launch_bounds__(kRunThreads, 3) k_run_sums(RunSums a, const T* __restrict__ grad, T* __restrict__ out) {
-    __shared__ float heads[kRunThreads * V];  // [group][V * lanes]
-    __shared__ uint8_t goes_on[kRunThreads];  // the group is one run, from before its first place to after its last
+    __shared__ float heads[kRunThreads * V * M];  // [vector][group][V * lanes]
+    __shared__ uint8_t goes_on[kRunThreads];      // the group is one run, from before its first place to after its last
     const uint32_t groups = kRunThreads / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x & (a.lanes - 1);
-    const uint32_t c = (blockIdx.y * a.lanes + lane) * V;
-    const bool column = c < a.dim;
+    uint32_t c[M];
+    bool column[M];
+    const T* from[M];
+#pragma unroll
+    for (int m = 0; m < M; m++) {
+        c[m] = ((blockIdx.y * M + m) * a.lanes + lane) * V;
+        column[m] = c[m] < a.dim;
+        from[m] = grad + (column[m] ? c[m] : 0);
+    }
     const uint64_t begin = ((uint64_t)blockIdx.x * groups + group) * a.chunk;
-    const T* from = grad + (column ? c : 0);
     cudaGridDependencySynchronize();  // the sorted list, and the cleared output
     uint32_t cur = key_at(a, begin);
     const bool from_before = begin > 0 && cur < a.vocab && key_at(a, begin - 1) == cur;
     bool head = from_before;  // the current run is the one that came in
-    Sums<V> acc;
-    acc.clear();
+    Sums<V> acc[M];
+#pragma unroll
+    for (int m = 0; m < M; m++) acc[m].clear();
+    auto keep_head = [&] {
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+#pragma unroll
+            for (int i = 0; i < V; i++) heads[(m * kRunThreads + threadIdx.x) * V + i] = acc[m].v[i];
+        }
+    };
+    auto write = [&](uint32_t key, const Sums<V>* sum) {
+#pragma unroll
+        for (int m = 0; m < M; m++)
+            if (column[m]) write_row<T, V>(a, out, key, c[m], sum[m]);
+    };
     // every place of the chunk holds a token: nothing to check
     const bool whole = begin + a.chunk <= a.count && a.items[begin + a.chunk - 1].x < a.vocab;
     auto batches = [&](auto checked) {
         constexpr bool kChecked = decltype(checked)::value;
         for (uint32_t p = 0; p < a.chunk; p += kAhead) {
             uint32_t key[kAhead], row[kAhead];
-            Pack<T, V> g[kAhead];
+            Pack<T, V> g[kAhead][M];
 #pragma unroll
             for (int k = 0; k < kAhead; k += 2) {  // the list has room for the last pair
                 const uint64_t i = begin + p + k;
@@ -621,62 +640,65 @@ __global__ void __launch_bounds__(kRunThreads, 3) k_run_sums(RunSums a, const T*
                 }
             }
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) g[k] = *reinterpret_cast<const Pack<T, V>*>(from + row[k] * a.grad_stride);
+            for (int k = 0; k < kAhead; k++) {
+#pragma unroll
+                for (int m = 0; m < M; m++)
+                    g[k][m] = *reinterpret_cast<const Pack<T, V>*>(from[m] + row[k] * a.grad_stride);
+            }
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
                 if (key[k] != cur) {
-                    if (head) {
-#pragma unroll
-                        for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc.v[i];
-                    } else if (column) {
-                        write_row<T, V>(a, out, cur, c, acc);
-                    }
+                    if (head) keep_head();
+                    else write(cur, acc);
                     head = false;
                     cur = key[k];
-                    acc.clear();
+#pragma unroll
+                    for (int m = 0; m < M; m++) acc[m].clear();
                 }
-                acc.add(g[k]);
+#pragma unroll
+                for (int m = 0; m < M; m++) acc[m].add(g[k][m]);
             }
         }
     };
     if (whole) batches(std::false_type{});
     else batches(std::true_type{});
     const bool to_after = cur < a.vocab && key_at(a, begin + a.chunk) == cur;
-    if (head) {
-#pragma unroll
-        for (int i = 0; i < V; i++) heads[threadIdx.x * V + i] = acc.v[i];
-    } else if (!to_after && cur < a.vocab && column) {
-        write_row<T, V>(a, out, cur, c, acc);
-    }
+    if (head) keep_head();
+    else if (!to_after && cur < a.vocab) write(cur, acc);
     if (lane == 0) goes_on[group] = head && to_after;
     __syncthreads();
     const uint64_t block = (uint64_t)blockIdx.x * 2 * a.dim;
+    auto add_head = [&](Sums<V>* sum, uint32_t h) {
+#pragma unroll
+        for (int m = 0; m < M; m++) sum[m].add(heads + (m * kRunThreads + h * a.lanes + lane) * V);
+    };
+    auto keep_part = [&](uint64_t at, const Sums<V>* sum) {
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            if (!column[m]) continue;
+#pragma unroll
+            for (int i = 0; i < V; i++) a.part[at + c[m] + i] = sum[m].v[i];
+        }
+    };
     if (!head && to_after) {  // a run that began here
-        uint32_t h = group + 1;
         bool open = true;
-        for (; h < groups && open; h++) {
-            acc.add(heads + (h * a.lanes + lane) * V);
+        for (uint32_t h = group + 1; h < groups && open; h++) {
+            add_head(acc, h);
             open = goes_on[h];
         }
-        if (column) {
-            if (open) {
-#pragma unroll
-                for (int i = 0; i < V; i++) a.part[block + a.dim + c + i] = acc.v[i];
-            } else {
-                write_row<T, V>(a, out, cur, c, acc);
-            }
-        }
+        if (open) keep_part(block + a.dim, acc);
+        else write(cur, acc);
     }
-    if (group == 0 && from_before && column) {  // the run that came into the block
-        Sums<V> sum;
-        sum.clear();
+    if (group == 0 && from_before) {  // the run that came into the block
+        Sums<V> sum[M];
+#pragma unroll
+        for (int m = 0; m < M; m++) sum[m].clear();
         bool open = true;
         for (uint32_t h = 0; h < groups && open; h++) {
-            sum.add(heads + (h * a.lanes + lane) * V);
+            add_head(sum, h);
             open = goes_on[h];
         }
-#pragma unroll
-        for (int i = 0; i < V; i++) a.part[block + c + i] = sum.v[i];
+        keep_part(block, sum);
     }
 }
 
@@ -736,6 +758,10 @@ template <class T, class F> void with_width(uint32_t v, F&& f) {
     else if (v == 4) f(std::integral_constant<int, 4>{});
     else f(std::integral_constant<int, kMost>{});
 }
+// Vectors that a lane of k_run_sums takes of a row: four where each is a single element (a row off the wider
+// boundaries), so that a place's key and row serve four loads.  8192 rows of 200 tokens of 127 bf16: 163 us, 220 with
+// one; pairs of 16-bit elements gain nothing.
+uint32_t vectors_of_lane(uint32_t v, uint32_t vectors) { return v == 1 && vectors > 8 ? 4 : 1; }
 // Launches a kernel that may be set up while the one before it on the stream
 // ends; it waits for that one (cudaGridDependencySynchronize) before it reads
 // anything.  Saves about 2 us a kernel where each takes a few.
@@ -988,11 +1014,12 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
             a.count = ws.count;
             a.vocab = (uint32_t)vocab;
             a.dim = dim;
-            a.lanes = lanes_for((dim + v - 1) / v);
+            const uint32_t vectors = (dim + v - 1) / v, each = vectors_of_lane(v, vectors);
+            a.lanes = lanes_for(ceil_div(vectors, each));
             a.grad_stride = grad_stride;
             a.out_stride = out_stride;
             a.scale = scale;
-            const uint32_t groups = kRunThreads / a.lanes, slices = ceil_div(dim, a.lanes * v);
+            const uint32_t groups = kRunThreads / a.lanes, slices = ceil_div(vectors, a.lanes * each);
             // longer chunks mean fewer joins, as long as every SM has a few blocks
             a.chunk = kMostChunk;
             while (a.chunk > kAhead && (uint64_t)ceil_div(ws.count, groups * a.chunk) * slices < kFewBlocks) a.chunk /= 2;
@@ -1001,9 +1028,12 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
                 using T = decltype(e);
                 with_width<T>(v, [&](auto wd) {
                     constexpr int V = decltype(wd)::value;
-                    launch_behind(k_run_sums<T, V>, grid, kRunThreads, s, a, static_cast<const T*>(grad),
-                                  static_cast<T*>(out));
-                    if (grid.x > 1) launch_behind(k_run_joins<T, V>, grid, kRunThreads, s, a, static_cast<T*>(out));
+                    constexpr int M = V == 1 ? 4 : 1;
+                    launch_behind(each == M ? k_run_sums<T, V, M> : k_run_sums<T, V, 1>, grid, kRunThreads, s, a,
+                                  static_cast<const T*>(grad), static_cast<T*>(out));
+                    if (grid.x > 1)
+                        launch_behind(k_run_joins<T, V>, dim3(grid.x, ceil_div(vectors, a.lanes)), kRunThreads, s, a,
+                                      static_cast<T*>(out));
                 });
             });
             FB_CUDA_CHECK(cudaGetLastError());
