@@ -1109,13 +1109,21 @@ template <class T> uint32_t steps_of(uint32_t classes, uint32_t warps) {
     return ceil_div(classes + 16 / sizeof(T) - 1, warps * 128);
 }
 
-template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(const SampleArgs& a) {
+// `most`: the classes of the longest row that the variant is launched for.  The
+// kernel's shared memory limit is one for all threads of the process, so it is
+// always set to what those need: a call that set it to its own size could come
+// between another thread's setting and launch.
+template <class T, bool HELD, int WARPS, int CTAS, int BLOCKS> void launch_row(const SampleArgs& a, uint32_t most = 0) {
     using Sh = RowShared<WARPS, CTAS>;
     const uint32_t steps = steps_of<T>(a.classes, WARPS * CTAS);
-    const size_t bytes = sizeof(Sh) + (HELD ? (size_t)WARPS * steps * 128 * sizeof(T) : 0);
+    auto bytes_for = [](uint32_t warp_steps) {
+        return sizeof(Sh) + (HELD ? (size_t)WARPS * warp_steps * 128 * sizeof(T) : 0);
+    };
+    const size_t bytes = bytes_for(steps);
     const auto kernel = k_sample_row<T, HELD, WARPS, CTAS, BLOCKS>;
     if (bytes > 48 << 10)
-        FB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        FB_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)bytes_for(steps_of<T>(most, WARPS * CTAS))));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((uint32_t)std::min<uint64_t>(1u << 18, a.n) * CTAS);
     cfg.blockDim = dim3(32 * WARPS);
@@ -1168,14 +1176,14 @@ template <class T> void launch_sample(const SampleArgs& a) {
     else if (k <= 64) launch_lanes<T, 2, 32>(a);
     else if (k <= 128) launch_lanes<T, 4, 32>(a);
     else if (k <= 256) launch_lanes<T, 8, 32>(a);
-    else if (k <= 512 && a.n >= 2048) launch_row<T, true, 1, 1, 20>(a);
-    else if (k <= 2048 && a.n >= 1024) launch_row<T, true, 2, 1, 16>(a);
-    else if (k <= 2048) launch_row<T, true, 4, 1, 8>(a);
-    else if (k <= 8192) launch_row<T, true, 8, 1, 4>(a);
-    else if (k > 32768 && a.n <= 8 && k <= 262144) launch_row<T, true, 16, 8, 1>(a);  // up to 128 KB a block
+    else if (k <= 512 && a.n >= 2048) launch_row<T, true, 1, 1, 20>(a, 512);
+    else if (k <= 2048 && a.n >= 1024) launch_row<T, true, 2, 1, 16>(a, 2048);
+    else if (k <= 2048) launch_row<T, true, 4, 1, 8>(a, 2048);
+    else if (k <= 8192) launch_row<T, true, 8, 1, 4>(a, 8192);
+    else if (k > 32768 && a.n <= 8 && k <= 262144) launch_row<T, true, 16, 8, 1>(a, 262144);  // up to 136 KB a block
     else if (k > 32768 && a.n <= 8) launch_row<T, false, 16, 8, 1>(a);
     else if (a.n <= 148) launch_row<T, false, 32, 1, 1>(a);
-    else if (k * sizeof(T) <= 65536) launch_row<T, true, 16, 1, 2>(a);
+    else if (k * sizeof(T) <= 65536) launch_row<T, true, 16, 1, 2>(a, 65536 / sizeof(T));
     else if (a.n <= 296 && unequal) launch_row<T, false, 32, 1, 1>(a);
     else launch_row<T, false, 16, 1, 2>(a);
 }

@@ -1,0 +1,83 @@
+"""ops called from several host threads and in one graph, at several sizes."""
+import ctypes as C
+import threading
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+# n, classes and type of draws that take the same kernel with different amounts of shared memory
+PAIRS = [
+    ((40, 8000, "float32"), (40, 6100, "float32")),          # a block a row
+    ((2, 200001, "float32"), (2, 40000, "float32")),         # a cluster a row
+    ((160, 32768, "bfloat16"), (160, 20001, "bfloat16")),    # a batch of long rows, a block each
+]
+
+
+def ops():
+    from ferrisboost_b200 import ops as o
+    return o
+
+
+def scores_of(n, classes, dtype, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((n, classes), generator=gen, device="cuda").to(getattr(torch, dtype))
+    return x, torch.rand(n, generator=gen, device="cuda")
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+def test_two_threads_draw_from_rows_of_two_lengths(pair):
+    """Calls of the C entry, which does not hold the interpreter's lock."""
+    from ferrisboost_b200 import _lib
+    entry = _lib.load().fbgpu_sample
+    inputs = [scores_of(*shape, seed) for seed, shape in enumerate(pair)]
+    want = [ops().sample(x, u, top_p=0.9) for x, u in inputs]
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(2)
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        x, u = inputs[i]
+        classes, probs = (torch.empty_like(t) for t in want[i])
+        params = _lib.FbgpuSampleParams(1.0, 0, 0.9, 0.0, None, None, None, None)
+        args = (C.c_void_p(x.data_ptr()), {"float32": 0, "bfloat16": 2}[pair[i][2]], len(x), x.shape[1], x.stride(0),
+                C.c_void_p(u.data_ptr()), C.byref(params), C.c_void_p(classes.data_ptr()), C.c_void_p(probs.data_ptr()),
+                C.c_void_p(stream.cuda_stream))
+        start.wait()
+        failed = sum(entry(*args) != 0 for _ in range(5000))
+        stream.synchronize()
+        if failed:
+            wrong.append(f"{failed} calls with {pair[i]} failed")
+        if not (torch.equal(classes, want[i][0]) and torch.equal(probs, want[i][1])):
+            wrong.append(f"another draw with {pair[i]}")
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_rows_of_several_lengths_in_one_graph():
+    shapes = [shape for pair in PAIRS for shape in pair]
+    inputs = [scores_of(*shape, seed) for seed, shape in enumerate(shapes)]
+
+    def step():
+        return [t for x, u in inputs for t in ops().sample(x, u, top_p=0.9)]
+
+    want = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(2):
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        for x, u in inputs:  # the last one is short
+            ops().sample(x, u, top_p=0.9)
