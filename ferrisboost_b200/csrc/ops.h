@@ -153,7 +153,9 @@ inline cudaStream_t check_stream(void* stream) {
     return s;
 }
 
-// The C boundary: no exception leaves it.
+// The C boundary: no exception leaves it, and no error of the runtime that it
+// reports: the runtime keeps a failed call's error for the thread's next check,
+// which would report it for work that ran.
 template <class F> fbgpu_status ops_guarded(F&& f) {
     try {
         f();
@@ -162,6 +164,7 @@ template <class F> fbgpu_status ops_guarded(F&& f) {
         noalloc_set_error(ex.what());
         return FBGPU_EINPUT;
     } catch (const CudaError& ex) {
+        cudaGetLastError();
         noalloc_set_error(ex.what());
         return FBGPU_ECUDA;
     } catch (const std::exception& ex) {

@@ -1,4 +1,5 @@
-"""ops called from several host threads and in one graph, at several sizes."""
+"""ops called from several host threads and in one graph at several
+sizes, and after a call that failed: a right call is not refused for another one."""
 import ctypes as C
 import threading
 
@@ -81,3 +82,25 @@ def test_rows_of_several_lengths_in_one_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, want))
         for x, u in inputs:  # the last one is short
             ops().sample(x, u, top_p=0.9)
+
+
+def test_a_call_after_one_that_failed():
+    """A launch into a capture that a query has ended fails on the host; the
+    thread's next call does not report that failure again."""
+    rt = C.CDLL("libcudart.so.12")
+    x, u = scores_of(3, 700, "float32", 1)
+    out = dict(classes=torch.empty(3, dtype=torch.int32, device="cuda"), probs=torch.empty(3, device="cuda"))
+    want = ops().dropout(x, 0.5, 1)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    handle = C.c_void_p(side.cuda_stream)
+    assert rt.cudaStreamBeginCapture(handle, 2) == 0  # relaxed: other streams and threads are not held back
+    assert rt.cudaStreamQuery(handle) != 0            # not allowed on a capturing stream, and ends the capture
+    with torch.cuda.stream(side):
+        with pytest.raises(RuntimeError, match="CUDA error"):
+            ops().sample(x, u, **out)
+    graph = C.c_void_p()
+    assert rt.cudaStreamEndCapture(handle, C.byref(graph)) != 0
+    rt.cudaGetLastError()
+    assert torch.equal(ops().dropout(x, 0.5, 1), want)
+    side.synchronize()
