@@ -75,7 +75,10 @@ template <int V> struct Sums {
 // threads takes four rows at a time, so that four loads are in flight and a
 // token is read once a row.  131072 random rows of 1024 bf16 out of 65534: 90 us,
 // 4.5 TB/s of what moves at least once (the table passes the L2 twice).
+// Columns are counted in 32 bits, and a lane steps past the last one: wider rows
+// are looked up kLookupColumns at a time.
 constexpr int kLookupThreads = 256, kLookupRows = 4;
+constexpr uint32_t kLookupColumns = 1u << 29;
 
 struct LookupArgs {
     uint64_t table_stride, n, out_stride;
@@ -857,31 +860,36 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
                 throw InputError("out must not overlap the table or the tokens");
             cudaStream_t s = check_stream(stream);
             if (!n || !dim) return;
-            const uint32_t v = vector_width(size, dim, table, table_stride, out, out_stride), vectors = (dim + v - 1) / v;
+            const uint32_t v = vector_width(size, dim, table, table_stride, out, out_stride);
             const Tokens<Tok> tk(tokens, token_row, token_col, vocab);
             if (per_row == 1) {
-                // rows of several 16-byte vectors that do not keep their boundaries
-                const bool odd = v * size < 16 && dim >= 64 / size && dim < 1u << 30;
-                LookupArgs a{table_stride, n, out_stride, dim, 0, scale};
-                while (1u << a.lanes_log < lanes_for(odd ? dim / (16 / size) + 2 : vectors)) a.lanes_log++;
-                // every SM full once, then several rows a group, then more
-                const uint64_t wish = (n + (kLookupThreads >> a.lanes_log) - 1) / (kLookupThreads >> a.lanes_log);
-                const uint64_t full = 148 * 8;
-                const uint32_t blocks = (uint32_t)std::min<uint64_t>(
-                    1u << 20, std::max(std::min(wish, full), (wish + kLookupRows - 1) / kLookupRows));
-                with_type(type, [&](auto e) {
-                    using T = decltype(e);
-                    if (odd) {
-                        k_lookup_odd<T, Tok><<<blocks, kLookupThreads, 0, s>>>(a, static_cast<const T*>(table), tk,
-                                                                              static_cast<T*>(out));
-                        return;
-                    }
-                    with_width<T>(v, [&](auto w) {
-                        k_lookup<T, Tok, decltype(w)::value><<<blocks, kLookupThreads, 0, s>>>(
-                            a, static_cast<const T*>(table), tk, static_cast<T*>(out));
+                for (uint64_t c = 0; c < dim; c += kLookupColumns) {
+                    const uint32_t columns = (uint32_t)std::min<uint64_t>(dim - c, kLookupColumns);
+                    // rows of several 16-byte vectors that do not keep their boundaries
+                    const bool odd = v * size < 16 && columns >= 64 / size;
+                    LookupArgs a{table_stride, n, out_stride, columns, 0, scale};
+                    while (1u << a.lanes_log < lanes_for(odd ? columns / (16 / size) + 2 : columns / v)) a.lanes_log++;
+                    // every SM full once, then several rows a group, then more
+                    const uint64_t wish = (n + (kLookupThreads >> a.lanes_log) - 1) / (kLookupThreads >> a.lanes_log);
+                    const uint64_t full = 148 * 8;
+                    const uint32_t blocks = (uint32_t)std::min<uint64_t>(
+                        1u << 20, std::max(std::min(wish, full), (wish + kLookupRows - 1) / kLookupRows));
+                    count_launch();
+                    with_type(type, [&](auto e) {
+                        using T = decltype(e);
+                        const T* from = static_cast<const T*>(table) + c;
+                        T* to = static_cast<T*>(out) + c;
+                        if (odd) {
+                            k_lookup_odd<T, Tok><<<blocks, kLookupThreads, 0, s>>>(a, from, tk, to);
+                            return;
+                        }
+                        with_width<T>(v, [&](auto w) {
+                            k_lookup<T, Tok, decltype(w)::value><<<blocks, kLookupThreads, 0, s>>>(a, from, tk, to);
+                        });
                     });
-                });
+                }
             } else {
+                const uint32_t vectors = dim / v;
                 BagArgs a{table_stride, n, out_stride, dim, per_row, per_row, 0, 0, scale};
                 while (1u << a.lanes_log < lanes_for(vectors)) a.lanes_log++;
                 const uint32_t slices = ceil_div(vectors, 1u << a.lanes_log);
@@ -894,6 +902,7 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
                 }
                 const uint32_t rows = kBagThreads >> (a.lanes_log + a.parts_log);
                 const dim3 grid((uint32_t)std::min<uint64_t>(1u << 20, (n + rows - 1) / rows), slices);
+                count_launch();
                 with_type(type, [&](auto e) {
                     using T = decltype(e);
                     with_width<T>(v, [&](auto w) {
@@ -906,7 +915,6 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
                     });
                 });
             }
-            count_launch();
             FB_CUDA_CHECK(cudaGetLastError());
         });
     });
