@@ -217,7 +217,8 @@ __global__ void __launch_bounds__(kBagThreads, 4) k_embed(BagArgs a, const T* __
     const uint32_t part = threadIdx.x >> a.lanes_log & ((1u << a.parts_log) - 1);
     const uint32_t rows = kBagThreads >> (a.lanes_log + a.parts_log);  // of a block
     const uint32_t c = (((uint32_t)blockIdx.y << a.lanes_log) + lane) * V;
-    const uint32_t begin = min(part * a.part_len, a.per_row), end = min(begin + a.part_len, a.per_row);
+    // `begin` + part_len may pass 2^32, begin + what is left of the row does not
+    const uint32_t begin = min(part * a.part_len, a.per_row), end = begin + min(a.part_len, a.per_row - begin);
     for (uint64_t r0 = (uint64_t)blockIdx.x * rows; r0 < a.n; r0 += (uint64_t)gridDim.x * rows) {
         const uint64_t r = r0 + (threadIdx.x >> (a.lanes_log + a.parts_log));
         Sums<V> sum;

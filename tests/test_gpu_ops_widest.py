@@ -24,3 +24,13 @@ def test_lookup_of_the_widest_rows(dim):
     for c in range(0, dim, part):
         assert torch.equal(flat[c:min(c + part, dim)], table[0, c:c + part]), c
     assert (flat[dim:] == 9.0).all()
+
+
+def test_the_longest_list_of_tokens():
+    """One row of 2^32 - 1 tokens (17 GB), summed in 256 parts of 2^24: the last part ends one token short of that,
+    and the token behind the row is not one of its own."""
+    buffer = torch.full((1 << 32,), -1, dtype=torch.int32, device="cuda")
+    buffer[0] = buffer[(1 << 32) - 2] = 0
+    buffer[(1 << 32) - 1] = 1
+    table = torch.tensor([[1.0], [100.0]], device="cuda")
+    assert ops().embed(table, buffer[:-1].view(1, -1)).item() == 2.0
