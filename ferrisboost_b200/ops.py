@@ -11,8 +11,10 @@ new ones, or fill ``out``.  Like torch's own operations they are enqueued on the
 current stream of the tensors' device and do not wait for it; a tensor made on
 another stream needs the usual ``wait_stream`` / ``record_stream``.  They can be
 captured into a CUDA graph.  They do not record gradients: a training step calls
-the backward operators itself (examples/leaf_head.py).  Wrong arguments raise
-ValueError before anything is enqueued.  The kernels are ``fbgpu_embed``, ``fbgpu_embed_grad``,
+the backward operators itself (examples/leaf_head.py).  A tensor that asks for a
+gradient is refused while torch records gradients (pass ``t.detach()``, or call
+under ``torch.no_grad()``).  Wrong arguments raise ValueError before anything is
+enqueued.  The kernels are ``fbgpu_embed``, ``fbgpu_embed_grad``,
 ``fbgpu_dropout`` and ``fbgpu_sample`` of include/fbgpu.h, which has the exact
 definitions; there is no CPU path.
 """
@@ -36,11 +38,19 @@ _entry = _lib.load()
 _device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
+def _no_grad(name: str, t: torch.Tensor) -> None:
+    """Refuses a tensor whose gradient would be lost without a word."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and no gradient is recorded here: pass it detached, or call under "
+                         "torch.no_grad()")
+
+
 def _type(name: str, t: Any, dims: int | None, types: dict) -> int:
     """The type code of a CUDA tensor, with its dimensions checked."""
     if isinstance(t, torch.Tensor):
         code = types.get(t.dtype)
         if code is not None and t.is_cuda and (dims is None or t.dim() == dims):
+            _no_grad(name, t)
             return code
         if not t.is_cuda:
             raise ValueError(f"{name} must be on a CUDA device, it is on {t.device}")
@@ -67,6 +77,7 @@ def _out(out: Any, shape: tuple, like: torch.Tensor) -> torch.Tensor:
     if not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != like.dtype:
         raise ValueError(f"out must be a {like.dtype} tensor of shape {shape}")
     _same_device("out", out, like.get_device())
+    _no_grad("out", out)
     return out
 
 
@@ -183,6 +194,7 @@ def _limit(name: str, value: Any, scores: torch.Tensor, dtype: torch.dtype) -> t
     if value.dtype != dtype or value.shape != scores.shape[:1] or not value.is_contiguous():
         raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {scores.shape[0]} values")
     _same_device(name, value, scores.get_device())
+    _no_grad(name, value)
     return 0, value.data_ptr()
 
 
@@ -190,6 +202,7 @@ def _result(name: str, t: Any, u: torch.Tensor, dtype: torch.dtype) -> torch.Ten
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != u.shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {u.shape[0]} values")
     _same_device(name, t, u.get_device())
+    _no_grad(name, t)
     return t
 
 
