@@ -13,8 +13,9 @@ another stream needs the usual ``wait_stream`` / ``record_stream``.  They can be
 captured into a CUDA graph.  They do not record gradients: a training step calls
 the backward operators itself (examples/leaf_head.py).  A tensor that asks for a
 gradient is refused while torch records gradients (pass ``t.detach()``, or call
-under ``torch.no_grad()``).  Wrong arguments raise ValueError before anything is
-enqueued.  The kernels are ``fbgpu_embed``, ``fbgpu_embed_grad``,
+under ``torch.no_grad()``), and what is written to ``out`` counts as an in-place
+change of it.  Wrong arguments raise ValueError before anything is enqueued.  The
+kernels are ``fbgpu_embed``, ``fbgpu_embed_grad``,
 ``fbgpu_dropout`` and ``fbgpu_sample`` of include/fbgpu.h, which has the exact
 definitions; there is no CPU path.
 """
@@ -93,6 +94,13 @@ def _call(device: int, f: Any, *args: Any) -> None:
         raise (ValueError if status == 1 else RuntimeError)(message)
 
 
+def _wrote(*given: torch.Tensor | None) -> None:
+    """Counts the write to the caller's own tensors, so that autograd sees a change of one that it has saved."""
+    for t in given:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
+
+
 def _token_shape(tokens: torch.Tensor) -> tuple:
     """(token code, rows, tokens per row, row stride, column stride)"""
     code = _type("tokens", tokens, None, _TOKENS)
@@ -126,9 +134,11 @@ def embed(table: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0,
     _same_device("tokens", tokens, device)
     vocab, dim = table.shape
     _count(dim, k)
+    given = out
     out = table.new_empty((n, dim)) if out is None else _out(out, (n, dim), table)
     _call(device, _entry.fbgpu_embed, table.data_ptr(), code, vocab, dim, _rows("table", table), tokens.data_ptr(), tcode, n,
           k, trow, tcol, scale, out.data_ptr(), _rows("out", out))
+    _wrote(given)
     return out
 
 
@@ -152,11 +162,13 @@ def embed_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale: f
         raise ValueError(f"grad has {grad.shape[0]} rows, tokens has {n}")
     dim = grad.shape[1]
     _count(dim, k)
+    given = out
     out = grad.new_empty((vocab, dim)) if out is None else _out(out, (vocab, dim), grad)
     size = _entry.fbgpu_embed_grad_workspace(n, k, vocab, dim)
     space = grad.new_empty(size, dtype=torch.uint8)
     _call(device, _entry.fbgpu_embed_grad, grad.data_ptr(), code, n, k, dim, _rows("grad", grad), tokens.data_ptr(), tcode,
           trow, tcol, vocab, scale, out.data_ptr(), _rows("out", out), space.data_ptr(), size)
+    _wrote(given)
     return out
 
 
@@ -172,6 +184,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, *,
     contiguous rows.  ``out=x`` works in place."""
     code = _type("x", x, None, _TYPES)
     p = float(p)
+    given = out
     out = x.new_empty(x.shape) if out is None else _out(out, tuple(x.shape), x)
     if x.is_contiguous() and out.is_contiguous():
         n, dim = 1, x.numel()
@@ -184,6 +197,7 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, *,
                          f"and strides {x.stride()}")
     _call(x.get_device(), _entry.fbgpu_dropout, x.data_ptr(), code, n, dim, xs, p, seed & 0xFFFFFFFFFFFFFFFF,
           offset & 0xFFFFFFFFFFFFFFFF, out.data_ptr(), os)
+    _wrote(given)
     return out
 
 
@@ -239,9 +253,11 @@ def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: Any = 1.0, top
         raise ValueError(f"top_k must be a whole number in 0..2**31 - 1, got {tk}")
     if k > 1 << 20:
         raise ValueError(f"classes must be in 2..1048576, got {k}")
+    given = classes, probs
     classes = u.new_empty(n, dtype=torch.int32) if classes is None else _result("classes", classes, u, torch.int32)
     probs = u.new_empty(n) if probs is None else _result("probs", probs, u, torch.float32)
     params = _lib.FbgpuSampleParams(t, int(tk), tp, mp, ts, tks, tps, mps)
     _call(device, _entry.fbgpu_sample, scores.data_ptr(), code, n, k, _rows("scores", scores), u.data_ptr(),
           C.byref(params), classes.data_ptr(), probs.data_ptr())
+    _wrote(*given)
     return classes, probs

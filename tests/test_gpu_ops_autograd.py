@@ -1,4 +1,5 @@
-"""ops next to autograd: no gradient is lost without a word."""
+"""ops next to autograd: no gradient is lost without a word, and a write to a
+tensor that autograd has saved is seen."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +43,30 @@ def test_and_taken_where_none_is_recorded():
             got = [call() for call in calls(y, tok, u)[:3] + calls(y, tok, u)[6:7]]
         assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(got, want))
         assert torch.equal(x, y)
+    with torch.inference_mode():  # a tensor without a count of its changes
+        z = torch.empty_like(x)
+        assert torch.equal(ops().dropout(x, 0.5, 1, out=z), want[2])
+
+
+def test_a_write_to_a_saved_tensor_is_seen():
+    x, tok, u = tensors()
+    f = dict(device="cuda")
+    writes = [
+        lambda h: ops().embed(x, tok, out=h), lambda h: ops().embed_grad(x, tok, 6, out=h),
+        lambda h: ops().dropout(h, 0.5, 1, out=h), lambda h: ops().sample(x, u, probs=h.view(-1)[:6]),
+    ]
+    for write in writes:
+        h = x.clone()
+        w = torch.ones_like(h).requires_grad_()
+        loss = (w * h).sum()  # saves h
+        write(h)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    classes = torch.empty(6, dtype=torch.int32, **f)
+    version = classes._version
+    ops().sample(x, u, classes=classes)
+    assert classes._version > version
+    # without out nothing that was there is touched
+    version = x._version
+    ops().dropout(x, 0.5, 1), ops().embed(x, tok), ops().sample(x, u)
+    assert x._version == version
