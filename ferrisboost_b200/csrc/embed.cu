@@ -10,7 +10,7 @@
 // equal parts, whatever the lengths of the tokens' runs.  A run inside a part is
 // written at once; what continues into another part is joined from the parts'
 // sums in a second pass.  No atomics: the order of every sum follows from the
-// tokens and the sizes.
+// tokens, the sizes and the element type, and is the same in every layout.
 #include <type_traits>
 
 #include <cooperative_groups.h>
@@ -590,17 +590,21 @@ template <class T, int V> __device__ __forceinline__ void write_row(const RunSum
     *reinterpret_cast<Pack<T, V>*>(out + key * a.out_stride + c) = sum.template scaled<T>(a.scale);
 }
 
-template <class T, int V, int M>  // M vectors of a lane, lanes apart
-__global__ void __launch_bounds__(kRunThreads, 3) k_run_sums(RunSums a, const T* __restrict__ grad, T* __restrict__ out) {
-    __shared__ float heads[kRunThreads * V * M];  // [vector][group][V * lanes]
+// M vectors of a lane, lanes apart; R times the threads and the lanes, for as many groups
+template <class T, int V, int M, int R>
+__global__ void __launch_bounds__(kRunThreads * R, R == 1 ? 3 : 2) k_run_sums(RunSums a, const T* __restrict__ grad,
+                                                                              T* __restrict__ out) {
+    constexpr int kThreads = kRunThreads * R;
+    __shared__ float heads[kThreads * V * M];     // [vector][group][V * lanes]
     __shared__ uint8_t goes_on[kRunThreads];      // the group is one run, from before its first place to after its last
-    const uint32_t groups = kRunThreads / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x & (a.lanes - 1);
+    const uint32_t lanes = a.lanes * R, groups = kThreads / lanes, group = threadIdx.x / lanes;
+    const uint32_t lane = threadIdx.x & (lanes - 1);
     uint32_t c[M];
     bool column[M];
     const T* from[M];
 #pragma unroll
     for (int m = 0; m < M; m++) {
-        c[m] = ((blockIdx.y * M + m) * a.lanes + lane) * V;
+        c[m] = ((blockIdx.y * M + m) * lanes + lane) * V;
         column[m] = c[m] < a.dim;
         from[m] = grad + (column[m] ? c[m] : 0);
     }
@@ -616,7 +620,7 @@ __global__ void __launch_bounds__(kRunThreads, 3) k_run_sums(RunSums a, const T*
 #pragma unroll
         for (int m = 0; m < M; m++) {
 #pragma unroll
-            for (int i = 0; i < V; i++) heads[(m * kRunThreads + threadIdx.x) * V + i] = acc[m].v[i];
+            for (int i = 0; i < V; i++) heads[(m * kThreads + threadIdx.x) * V + i] = acc[m].v[i];
         }
     };
     auto write = [&](uint32_t key, const Sums<V>* sum) {
@@ -674,7 +678,7 @@ __global__ void __launch_bounds__(kRunThreads, 3) k_run_sums(RunSums a, const T*
     const uint64_t block = (uint64_t)blockIdx.x * 2 * a.dim;
     auto add_head = [&](Sums<V>* sum, uint32_t h) {
 #pragma unroll
-        for (int m = 0; m < M; m++) sum[m].add(heads + (m * kRunThreads + h * a.lanes + lane) * V);
+        for (int m = 0; m < M; m++) sum[m].add(heads + (m * kThreads + h * lanes + lane) * V);
     };
     auto keep_part = [&](uint64_t at, const Sums<V>* sum) {
 #pragma unroll
@@ -762,10 +766,27 @@ template <class T, class F> void with_width(uint32_t v, F&& f) {
     else if (v == 4) f(std::integral_constant<int, 4>{});
     else f(std::integral_constant<int, kMost>{});
 }
-// Vectors that a lane of k_run_sums takes of a row: four where each is a single element (a row off the wider
+// The same of rows that keep 16-byte boundaries.  How a sum is split follows from this width, so that its order, and
+// with it every bit, depends on the sizes and the type alone; rows off the boundaries take narrower vectors in that split.
+uint32_t even_width(uint32_t size, uint64_t dim) { return vector_width(size, dim, nullptr, 0, nullptr, 0); }
+// Vectors that a lane of k_run_sums takes of an even row: four where each is a single element (a row off the wider
 // boundaries), so that a place's key and row serve four loads.  8192 rows of 200 tokens of 127 bf16: 163 us, 220 with
 // one; pairs of 16-bit elements gain nothing.
 uint32_t vectors_of_lane(uint32_t v, uint32_t vectors) { return v == 1 && vectors > 8 ? 4 : 1; }
+// f with constants M and R of k_run_sums, for vectors narrower than even ones: as many a lane as make up for it, up to
+// two pairs or four elements, then twice the lanes.  8192 rows of 200 tokens, a bf16 gradient one element off: 112 us for
+// rows of 32, 130 without the second; two off: 87 for rows of 32, 142 for 128 (110 and 189); even: 75 and 110.  Where
+// the lanes of an even row are a warp already, more of them cost single elements time (1024: 87 us, 81 without).
+template <class T, int V, class F> void with_vectors_of_lane(uint32_t each, uint32_t lanes, F&& f) {
+    using std::integral_constant;
+    constexpr int kEven = 16 / (int)sizeof(T) / V, kMost = V == 1 ? 4 : std::min(2, kEven);
+    if constexpr (kEven > kMost) {
+        if (each > kMost && (V > 1 || lanes < 32)) return f(integral_constant<int, kMost>{}, integral_constant<int, 2>{});
+    }
+    if (each > 2) f(integral_constant<int, kMost>{}, integral_constant<int, 1>{});
+    else if (each > 1) f(integral_constant<int, std::min(2, kMost)>{}, integral_constant<int, 1>{});
+    else f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+}
 // Launches a kernel that may be set up while the one before it on the stream
 // ends; it waits for that one (cudaGridDependencySynchronize) before it reads
 // anything.  Saves about 2 us a kernel where each takes a few.
@@ -890,17 +911,23 @@ extern "C" fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vo
                     });
                 }
             } else {
-                const uint32_t vectors = dim / v;
                 BagArgs a{table_stride, n, out_stride, dim, per_row, per_row, 0, 0, scale};
-                while (1u << a.lanes_log < lanes_for(vectors)) a.lanes_log++;
-                const uint32_t slices = ceil_div(vectors, 1u << a.lanes_log);
-                if (slices > kMostSlices) throw InputError("fbgpu_embed takes rows of at most 2097120 elements");
-                // parts of a row, until every SM has about a thousand threads; a part has at least eight tokens
-                while (a.lanes_log + a.parts_log < 8 && a.part_len > kBagAhead &&
-                       n < (148ull * 1024 >> (a.lanes_log + a.parts_log)) / slices) {
+                // parts of a row, until every SM has about a thousand threads; a part has at least eight tokens.  As for
+                // even rows in every layout: 8192 rows of 200 tokens of 32 bf16, one element off, take 47 us in eight
+                // parts (37 whole, in another order; even rows 21)
+                const uint32_t even = dim / even_width(size, dim), even_lanes = lanes_for(even);
+                uint32_t even_log = 0;
+                while (1u << even_log < even_lanes) even_log++;
+                const uint32_t even_slices = ceil_div(even, even_lanes);
+                while (even_log + a.parts_log < 8 && a.part_len > kBagAhead &&
+                       n < (148ull * 1024 >> (even_log + a.parts_log)) / even_slices) {
                     a.parts_log++;
                     a.part_len = ceil_div(per_row, 1u << a.parts_log);
                 }
+                const uint32_t vectors = dim / v;
+                while (a.lanes_log + a.parts_log < 8 && 1u << a.lanes_log < lanes_for(vectors)) a.lanes_log++;
+                const uint32_t slices = ceil_div(vectors, 1u << a.lanes_log);
+                if (slices > kMostSlices) throw InputError("fbgpu_embed takes rows of at most 2097120 elements");
                 const uint32_t rows = kBagThreads >> (a.lanes_log + a.parts_log);
                 const dim3 grid((uint32_t)std::min<uint64_t>(1u << 20, (n + rows - 1) / rows), slices);
                 count_launch();
@@ -1023,25 +1050,27 @@ extern "C" fbgpu_status fbgpu_embed_grad(const void* grad, int32_t type, uint64_
             a.count = ws.count;
             a.vocab = (uint32_t)vocab;
             a.dim = dim;
-            const uint32_t vectors = (dim + v - 1) / v, each = vectors_of_lane(v, vectors);
-            a.lanes = lanes_for(ceil_div(vectors, each));
+            const uint32_t even_v = even_width(size, dim), even = dim / even_v, even_each = vectors_of_lane(even_v, even);
+            a.lanes = lanes_for(ceil_div(even, even_each));
             a.grad_stride = grad_stride;
             a.out_stride = out_stride;
             a.scale = scale;
-            const uint32_t groups = kRunThreads / a.lanes, slices = ceil_div(vectors, a.lanes * each);
+            const uint32_t groups = kRunThreads / a.lanes, even_slices = ceil_div(even, a.lanes * even_each);
             // longer chunks mean fewer joins, as long as every SM has a few blocks
             a.chunk = kMostChunk;
-            while (a.chunk > kAhead && (uint64_t)ceil_div(ws.count, groups * a.chunk) * slices < kFewBlocks) a.chunk /= 2;
-            const dim3 grid(ceil_div(ws.count, groups * a.chunk), slices);
+            while (a.chunk > kAhead && (uint64_t)ceil_div(ws.count, groups * a.chunk) * even_slices < kFewBlocks) a.chunk /= 2;
+            const uint32_t blocks = ceil_div(ws.count, groups * a.chunk), vectors = dim / v;
             with_type(type, [&](auto e) {
                 using T = decltype(e);
                 with_width<T>(v, [&](auto wd) {
                     constexpr int V = decltype(wd)::value;
-                    constexpr int M = V == 1 ? 4 : 1;
-                    launch_behind(each == M ? k_run_sums<T, V, M> : k_run_sums<T, V, 1>, grid, kRunThreads, s, a,
-                                  static_cast<const T*>(grad), static_cast<T*>(out));
-                    if (grid.x > 1)
-                        launch_behind(k_run_joins<T, V>, dim3(grid.x, ceil_div(vectors, a.lanes)), kRunThreads, s, a,
+                    with_vectors_of_lane<T, V>(even_v * even_each / v, a.lanes, [&](auto m, auto r) {
+                        constexpr int M = decltype(m)::value, R = decltype(r)::value;
+                        launch_behind(k_run_sums<T, V, M, R>, dim3(blocks, ceil_div(vectors, a.lanes * M * R)),
+                                      kRunThreads * R, s, a, static_cast<const T*>(grad), static_cast<T*>(out));
+                    });
+                    if (blocks > 1)
+                        launch_behind(k_run_joins<T, V>, dim3(blocks, ceil_div(vectors, a.lanes)), kRunThreads, s, a,
                                       static_cast<T*>(out));
                 });
             });

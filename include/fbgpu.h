@@ -444,8 +444,8 @@ fbgpu_status fbgpu_explain_device(fbgpu_model* m, int32_t kind, const float* X, 
  * `dim` elements of `type`, summed in f32 and rounded once.  Token (r, j) is at
  * tokens + r * token_row + j * token_col; one outside [0, vocab) stands for a
  * missing value and adds nothing (a row of only such tokens is zero).  The
- * order of the sum depends on the sizes alone.  With several tokens a row, dim
- * is at most 2097120. */
+ * order of the sum depends on the sizes and the type alone, not on addresses
+ * or strides.  With several tokens a row, dim is at most 2097120. */
 fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vocab, uint32_t dim, uint64_t table_stride,
                          const void* tokens, int32_t token_type, uint64_t n, uint32_t per_row, uint64_t token_row,
                          uint64_t token_col, float scale, void* out, uint64_t out_stride, void* stream);
@@ -453,8 +453,9 @@ fbgpu_status fbgpu_embed(const void* table, int32_t type, uint64_t vocab, uint32
 /* The gradient of fbgpu_embed for its table: out[v] = scale * sum of grad[r]
  * over the places (r, j) that hold token v, vocab rows of `dim` elements,
  * every one written.  The places are sorted by token (stable), so that each
- * row is summed in f32 in an order that depends on the tokens alone, with no
- * atomics: the same inputs give the same bits.  grad's stride may be 0 (one row
+ * row is summed in f32 in an order that depends on the tokens, the sizes and the
+ * type alone, with no atomics: the same inputs give the same bits, whatever
+ * their addresses and strides.  grad's stride may be 0 (one row
  * for all).  n * per_row and vocab are at most 2^31 - 2, dim at most 2097120.  `workspace` holds
  * fbgpu_embed_grad_workspace(...) bytes, 256-byte aligned, with any contents. */
 uint64_t fbgpu_embed_grad_workspace(uint64_t n, uint32_t per_row, uint64_t vocab, uint32_t dim);
