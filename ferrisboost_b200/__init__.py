@@ -808,6 +808,9 @@ class Model:
         import torch
 
         from . import ops
+        ks = np.asarray(top_k)
+        if ks.ndim and not np.all((ks >= -2**31) & (ks < 2**31) & (ks == np.trunc(ks))):
+            raise ValueError("top_k must be whole numbers of 32 bits")  # a conversion would cut them off
         margins = self.predict(data, output_margin=True, device=device)
         dev = torch.device("cuda", self._device(device))
         u = np.ascontiguousarray(u, dtype=np.float32)

@@ -1,0 +1,33 @@
+"""Arguments of the operators on the Python side: what a conversion would
+change without a word is refused, what means the same is taken."""
+import types
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Predicted(Exception):
+    pass
+
+
+def model():
+    def predict(*args, **kw):
+        raise Predicted
+    return types.SimpleNamespace(num_outputs=3, predict=predict)
+
+
+@pytest.mark.parametrize("top_k", [[1.5, 2.0], [2**32 + 1, 5], np.array([2**31]), [float("nan")], [-2**31 - 1],
+                                   [float("inf"), 1.0]])
+def test_model_sample_refuses_top_k_that_is_no_int32(top_k):
+    from ferrisboost_b200 import Model
+    with pytest.raises(ValueError, match="top_k"):
+        Model.sample(model(), None, None, top_k=top_k)
+
+
+@pytest.mark.parametrize("top_k", [5, 0, [1, 2], [2.0, 3.0], np.array([2**31 - 1, -2**31]), np.array([3], np.uint8)])
+def test_model_sample_takes_whole_top_k(top_k):
+    from ferrisboost_b200 import Model
+    with pytest.raises(Predicted):  # the check is over
+        Model.sample(model(), None, None, top_k=top_k)
