@@ -22,6 +22,7 @@ definitions; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+from operator import index
 from typing import Any
 
 import torch
@@ -195,8 +196,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, *,
     else:
         raise ValueError(f"x and out must be contiguous, or 2-D with contiguous rows; x has shape {tuple(x.shape)} "
                          f"and strides {x.stride()}")
-    _call(x.get_device(), _entry.fbgpu_dropout, x.data_ptr(), code, n, dim, xs, p, seed & 0xFFFFFFFFFFFFFFFF,
-          offset & 0xFFFFFFFFFFFFFFFF, out.data_ptr(), os)
+    _call(x.get_device(), _entry.fbgpu_dropout, x.data_ptr(), code, n, dim, xs, p,
+          index(seed) & 0xFFFFFFFFFFFFFFFF, index(offset) & 0xFFFFFFFFFFFFFFFF, out.data_ptr(), os)
     _wrote(given)
     return out
 

@@ -31,3 +31,16 @@ def test_model_sample_takes_whole_top_k(top_k):
     from ferrisboost_b200 import Model
     with pytest.raises(Predicted):  # the check is over
         Model.sample(model(), None, None, top_k=top_k)
+
+
+@pytest.mark.gpu
+def test_numbers_of_numpy_are_numbers():
+    from ferrisboost_b200 import ops
+    x = torch.randn((5, 9), device="cuda")
+    want = ops.dropout(x, 0.5, -7, 11)
+    for kind in (np.int64, np.int32, np.int8):
+        assert torch.equal(ops.dropout(x, np.float32(0.5), kind(-7), kind(11)), want)
+    top = np.uint64(2**64 - 7)  # the same 64 bits
+    assert torch.equal(ops.dropout(x, 0.5, top, np.uint8(11)), want)
+    with pytest.raises(TypeError):
+        ops.dropout(x, 0.5, 1.5)
