@@ -250,7 +250,7 @@ def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: Any = 1.0, top
     tk, tks = _limit("top_k", top_k, scores, torch.int32)
     tp, tps = _limit("top_p", top_p, scores, torch.float32)
     mp, mps = _limit("min_p", min_p, scores, torch.float32)
-    if tks is None and (tk != int(tk) or not 0 <= tk < 1 << 31):
+    if tks is None and (not 0 <= tk < 1 << 31 or tk != int(tk)):
         raise ValueError(f"top_k must be a whole number in 0..2**31 - 1, got {tk}")
     if k > 1 << 20:
         raise ValueError(f"classes must be in 2..1048576, got {k}")

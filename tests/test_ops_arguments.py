@@ -44,3 +44,12 @@ def test_numbers_of_numpy_are_numbers():
     assert torch.equal(ops.dropout(x, 0.5, top, np.uint8(11)), want)
     with pytest.raises(TypeError):
         ops.dropout(x, 0.5, 1.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top_k", [float("inf"), float("nan"), -1, 2**31, 1.5])
+def test_sample_refuses_top_k(top_k):
+    from ferrisboost_b200 import ops
+    x = torch.zeros((5, 9), device="cuda")
+    with pytest.raises(ValueError, match="top_k"):
+        ops.sample(x, x[:, 0].contiguous(), top_k=top_k)
