@@ -40,9 +40,9 @@ _entry = _lib.load()
 _device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _no_grad(name: str, t: torch.Tensor) -> None:
-    """Refuses a tensor whose gradient would be lost without a word."""
-    if t.requires_grad and torch.is_grad_enabled():
+def _lost_gradient(name: str, t: torch.Tensor) -> None:
+    """Refuses a tensor that requires a gradient where that would be lost without a word."""
+    if torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, and no gradient is recorded here: pass it detached, or call under "
                          "torch.no_grad()")
 
@@ -52,7 +52,8 @@ def _type(name: str, t: Any, dims: int | None, types: dict) -> int:
     if isinstance(t, torch.Tensor):
         code = types.get(t.dtype)
         if code is not None and t.is_cuda and (dims is None or t.dim() == dims):
-            _no_grad(name, t)
+            if t.requires_grad:
+                _lost_gradient(name, t)
             return code
         if not t.is_cuda:
             raise ValueError(f"{name} must be on a CUDA device, it is on {t.device}")
@@ -79,7 +80,8 @@ def _out(out: Any, shape: tuple, like: torch.Tensor) -> torch.Tensor:
     if not isinstance(out, torch.Tensor) or tuple(out.shape) != shape or out.dtype != like.dtype:
         raise ValueError(f"out must be a {like.dtype} tensor of shape {shape}")
     _same_device("out", out, like.get_device())
-    _no_grad("out", out)
+    if out.requires_grad:
+        _lost_gradient("out", out)
     return out
 
 
@@ -95,11 +97,8 @@ def _call(device: int, f: Any, *args: Any) -> None:
         raise (ValueError if status == 1 else RuntimeError)(message)
 
 
-def _wrote(*given: torch.Tensor | None) -> None:
-    """Counts the write to the caller's own tensors, so that autograd sees a change of one that it has saved."""
-    for t in given:
-        if t is not None:
-            torch.autograd.graph.increment_version(t)
+# Counts a write to a caller's tensor, so that autograd sees a change of one that it has saved.
+_wrote = torch.autograd.graph.increment_version
 
 
 def _token_shape(tokens: torch.Tensor) -> tuple:
@@ -139,7 +138,8 @@ def embed(table: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0,
     out = table.new_empty((n, dim)) if out is None else _out(out, (n, dim), table)
     _call(device, _entry.fbgpu_embed, table.data_ptr(), code, vocab, dim, _rows("table", table), tokens.data_ptr(), tcode, n,
           k, trow, tcol, scale, out.data_ptr(), _rows("out", out))
-    _wrote(given)
+    if given is not None:
+        _wrote(given)
     return out
 
 
@@ -169,7 +169,8 @@ def embed_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale: f
     space = grad.new_empty(size, dtype=torch.uint8)
     _call(device, _entry.fbgpu_embed_grad, grad.data_ptr(), code, n, k, dim, _rows("grad", grad), tokens.data_ptr(), tcode,
           trow, tcol, vocab, scale, out.data_ptr(), _rows("out", out), space.data_ptr(), size)
-    _wrote(given)
+    if given is not None:
+        _wrote(given)
     return out
 
 
@@ -198,7 +199,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0, *,
                          f"and strides {x.stride()}")
     _call(x.get_device(), _entry.fbgpu_dropout, x.data_ptr(), code, n, dim, xs, p,
           index(seed) & 0xFFFFFFFFFFFFFFFF, index(offset) & 0xFFFFFFFFFFFFFFFF, out.data_ptr(), os)
-    _wrote(given)
+    if given is not None:
+        _wrote(given)
     return out
 
 
@@ -209,7 +211,8 @@ def _limit(name: str, value: Any, scores: torch.Tensor, dtype: torch.dtype) -> t
     if value.dtype != dtype or value.shape != scores.shape[:1] or not value.is_contiguous():
         raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {scores.shape[0]} values")
     _same_device(name, value, scores.get_device())
-    _no_grad(name, value)
+    if value.requires_grad:
+        _lost_gradient(name, value)
     return 0, value.data_ptr()
 
 
@@ -217,7 +220,8 @@ def _result(name: str, t: Any, u: torch.Tensor, dtype: torch.dtype) -> torch.Ten
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != u.shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {u.shape[0]} values")
     _same_device(name, t, u.get_device())
-    _no_grad(name, t)
+    if t.requires_grad:
+        _lost_gradient(name, t)
     return t
 
 
@@ -254,11 +258,12 @@ def sample(scores: torch.Tensor, u: torch.Tensor, *, temperature: Any = 1.0, top
         raise ValueError(f"top_k must be a whole number in 0..2**31 - 1, got {tk}")
     if k > 1 << 20:
         raise ValueError(f"classes must be in 2..1048576, got {k}")
-    given = classes, probs
+    given = [t for t in (classes, probs) if t is not None]
     classes = u.new_empty(n, dtype=torch.int32) if classes is None else _result("classes", classes, u, torch.int32)
     probs = u.new_empty(n) if probs is None else _result("probs", probs, u, torch.float32)
     params = _lib.FbgpuSampleParams(t, int(tk), tp, mp, ts, tks, tps, mps)
     _call(device, _entry.fbgpu_sample, scores.data_ptr(), code, n, k, _rows("scores", scores), u.data_ptr(),
           C.byref(params), classes.data_ptr(), probs.data_ptr())
-    _wrote(*given)
+    if given:
+        _wrote(given)
     return classes, probs
