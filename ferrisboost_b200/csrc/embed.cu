@@ -767,7 +767,8 @@ template <class T, class F> void with_width(uint32_t v, F&& f) {
     else f(std::integral_constant<int, kMost>{});
 }
 // The same of rows that keep 16-byte boundaries.  How a sum is split follows from this width, so that its order, and
-// with it every bit, depends on the sizes and the type alone; rows off the boundaries take narrower vectors in that split.
+// with it every bit, depends on the sizes and the type alone; rows off the boundaries take narrower vectors in that
+// split.
 uint32_t even_width(uint32_t size, uint64_t dim) { return vector_width(size, dim, nullptr, 0, nullptr, 0); }
 // Vectors that a lane of k_run_sums takes of an even row: four where each is a single element (a row off the wider
 // boundaries), so that a place's key and row serve four loads.  8192 rows of 200 tokens of 127 bf16: 163 us, 220 with

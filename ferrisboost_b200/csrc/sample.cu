@@ -927,9 +927,10 @@ template <class T, bool HELD, int WARPS, int CTAS> struct RowDraw {
                         above = s.pick_above;
                     }
                 } else {
-                    // More than a list holds: halve the range of their keys, reading the row.  All above `hi`
-                    // have the weight `above`, below the goal; with those from `lo` on it is reached.  The ends
-                    // are keys that occur.
+                    // More than a list holds, as in flat rows, whose scores lie within few bins: halve the range
+                    // of their keys, reading the row (1000 rows of 20000 normal f32 scores with top_p 0.9: 123 us
+                    // at deviation 2, 352 at 0.1; 577 at deviation 2 and T = 100).  All above `hi` have the weight
+                    // `above`, below the goal; with those from `lo` on it is reached.  The ends are keys that occur.
                     auto each_member = [&](auto&& f) {
                         each([&](float v) {
                             if (member(v)) f(key_of(score(v)));
